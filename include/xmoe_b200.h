@@ -337,6 +337,71 @@ int xmoe_forward_gated(const xmoe_config* cfg, const xmoe_weights* w, const void
                        void* logits_out, int32_t n_tokens, void* y, void* workspace, size_t workspace_bytes,
                        xmoe_stream_t stream);
 
+/* ---- tokens sorted by expert and back, for experts of any format, with gradients ----------------------- */
+/* No counterpart in the reference (its operator only sorts inside the quantiser and brings rows back unweighted).
+ * topk_row [n_tokens, idx_stride] (xmoe_route_pack): slot s < k of token t lives in row topk_row[t, s] of num_rows; an
+ * entry outside [0, num_rows) is a slot without a row. No two slots name the same row (a plan of xmoe_route_pack never
+ * does; xmoe_unpermute alone also takes plans that do). Rows that no slot names are left as they were. Element types:
+ * XMOE_BF16 / XMOE_FP16 / XMOE_FP32 for x, y, rows; XMOE_BF16 / XMOE_FP32 for the weights w [n_tokens, w_stride]. Sums in
+ * fp32, slot 0 first, rounded once; no atomics. Any hidden size; 16-byte accesses where rows are 16-byte aligned. */
+#define XMOE_BF16 0
+#define XMOE_FP16 1
+#define XMOE_FP32 2
+/* rows[topk_row[t, s]] = x[t] */
+int xmoe_permute(const void* x, const int32_t* topk_row, int32_t n_tokens, int32_t hidden, int32_t k, int32_t idx_stride,
+                 int32_t num_rows, int32_t dtype, void* rows, xmoe_stream_t stream);
+/* y[t] = sum_s w[t, s] * rows[topk_row[t, s]]; w NULL: unweighted (the gradient of xmoe_permute). */
+int xmoe_unpermute(const void* rows, const int32_t* topk_row, const void* w, int32_t w_dtype, int32_t w_stride,
+                   int32_t n_tokens, int32_t hidden, int32_t k, int32_t idx_stride, int32_t num_rows, int32_t dtype,
+                   void* y, xmoe_stream_t stream);
+/* drows[topk_row[t, s]] = w[t, s] * dy[t]; dw f32 [n_tokens, k]: <dy[t], rows[topk_row[t, s]]>, 0 for a slot without a
+ * row. drows must not overlap rows. */
+int xmoe_unpermute_backward(const void* dy, const void* rows, const int32_t* topk_row, const void* w, int32_t w_dtype,
+                            int32_t w_stride, int32_t n_tokens, int32_t hidden, int32_t k, int32_t idx_stride,
+                            int32_t num_rows, int32_t dtype, void* drows, float* dw, xmoe_stream_t stream);
+
+/* ---- 8-bit operands with one scale per block of 128, and their products --------------------------------- */
+/* No counterpart in the reference. Activations: e4m3 codes [rows, ldq] (ldq a multiple of 16, q 16-byte aligned) and
+ * fp32 scales BLOCK-MAJOR [ceil(cols / 128), lds] (lds >= rows, a multiple of 4, 16-byte aligned): value = code *
+ * scale[col / 128][row]. Weights: codes [mats, n, ldw] and scales [mats, ceil(n / 128), ceil(k / 128)], one per 128 x 128
+ * block, the layout of block-scaled FP8 checkpoints. scale = max|v| / 448, code = e4m3(v / scale), nearest, ties to even;
+ * a block of zeros has scale 0, a block holding an infinity or a NaN gets NaN codes. */
+/* Rows of x [rows, ldx]. topk_row NULL: row r of q is row r of x (num_rows, k unused). Otherwise as xmoe_permute: the codes
+ * and scales of token t go to the rows topk_row[t, s] of q [num_rows, ldq]. */
+int xmoe_fp8_quant(const void* x, int32_t dtype, int32_t rows, int32_t cols, int32_t ldx, const int32_t* topk_row, int32_t k,
+                   int32_t idx_stride, int32_t num_rows, void* q, int32_t ldq, float* scale, int32_t lds,
+                   xmoe_stream_t stream);
+/* Weights [mats, n, k], contiguous. */
+int xmoe_fp8_quant_weight(const void* w, int32_t dtype, int32_t mats, int32_t n, int32_t k, void* q, int32_t ldq,
+                          float* scale, xmoe_stream_t stream);
+/* The gated activation of h = gate | up [rows, 2 * inter], quantised: q [rows, ldq], scale [ceil(inter / 128), lds].
+ * activation, alpha and limit as in xmoe_config. counts / offsets [mats] / [mats + 1]: only each expert's live rows are
+ * read and written; NULL: all rows. */
+int xmoe_glu_fp8_quant(const void* h, int32_t dtype, int32_t rows, int32_t inter, int32_t activation, float alpha,
+                       float limit, const int32_t* counts, const int32_t* offsets, int32_t mats, void* q, int32_t ldq,
+                       float* scale, int32_t lds, xmoe_stream_t stream);
+/* dh [rows, 2 * inter] from the gradient da [rows, inter] of the (unquantised) activation. A clamped gate or up value
+ * (activation 1) has gradient 0 outside its limits. */
+int xmoe_glu_backward(const void* da, const void* h, int32_t dtype, int32_t rows, int32_t inter, int32_t activation,
+                      float alpha, float limit, const int32_t* counts, const int32_t* offsets, int32_t mats, void* dh,
+                      xmoe_stream_t stream);
+/* out[m, f], f < n: sum over k of x[m, k] * w[f, k] (scales applied; every 128-block's product is added in fp32).
+ * transpose != 0: the same stored weight contracted over its rows, out[m, f], f < k: sum over n of x[m, n] * w[n, f].
+ * x [rows, ldx] and its scales cover k (transpose: n) columns. out [rows, ldo] of out_dtype. */
+int xmoe_fp8_gemm(const void* x, int32_t ldx, const float* x_scale, int32_t lds, const void* w, int32_t ldw,
+                  const float* w_scale, int32_t rows, int32_t n, int32_t k, int32_t transpose, void* out, int32_t out_dtype,
+                  int32_t ldo, xmoe_stream_t stream);
+/* The same, where the rows [offsets[e], offsets[e] + counts[e]) meet matrix e (device arrays as xmoe_route_pack writes
+ * them; a segment must start at a multiple of 16). w: matrix e at byte e * w_mat_stride. Rows outside the segments are
+ * left as they were. rows_in_use: an upper bound of the sum of counts that picks the kernel's token tile (0: rows). */
+int xmoe_fp8_grouped_gemm(const void* x, int32_t ldx, const float* x_scale, int32_t lds, const void* w, int32_t ldw,
+                          int64_t w_mat_stride, const float* w_scale, const int32_t* counts, const int32_t* offsets,
+                          int32_t mats, int32_t rows, int32_t rows_in_use, int32_t n, int32_t k, int32_t transpose,
+                          void* out, int32_t out_dtype, int32_t ldo, xmoe_stream_t stream);
+/* Synchronises `stream`, returns and clears the current device's first error of the two products since the last call
+ * (codes as xmoe_read_status; 0x700: a segment outside the buffers or not at a multiple of 16, treated as empty). */
+int xmoe_fp8_status(uint32_t* host_out, xmoe_stream_t stream);
+
 /* Measurement aid, no reference counterpart: the rate at which this GPU retires tcgen05.mma
  * instructions of the largest shape (M 128, N 256) with operands resident on chip, one issuing
  * thread per SM, n_mma instructions each (rounded down to a multiple of 64; ~100000 runs for a

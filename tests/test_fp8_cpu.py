@@ -1,0 +1,126 @@
+"""Refusals of the operators around FP8 experts, and the plain forms the GPU tests compare with: no GPU needed."""
+import ctypes as C
+
+import pytest
+import torch
+
+from tests import fp8_plain as P
+from xcaliber_b200 import _lib, fp8, ops
+
+A = 1 << 20  # an aligned address that no refused call may touch
+ARG, SHAPE, LIMIT = 1, 2, 6
+
+
+@pytest.mark.parametrize("args,rc", [
+    ((A, A, -1, 64, 2, 2, 128, 0, A, None), ARG), ((None, A, 4, 64, 2, 2, 128, 0, A, None), ARG),
+    ((A, None, 4, 64, 2, 2, 128, 0, A, None), ARG), ((A, A, 4, 64, 2, 2, 128, 0, None, None), ARG),
+    ((A, A, 4, 0, 2, 2, 128, 0, A, None), SHAPE), ((A, A, 4, 64, 2, 1, 128, 0, A, None), SHAPE),
+    ((A, A, 4, 64, 2, 2, 128, 3, A, None), SHAPE), ((A, A, 4, 64, 2, 2, -1, 0, A, None), ARG),
+    ((None, None, 0, 64, 2, 2, 128, 0, None, None), 0), ((A, A, 4, 64, 2, 2, 0, 0, None, None), 0),
+])
+def test_permute_refuses(built_lib, args, rc):
+    assert built_lib.xmoe_permute(*args) == rc
+
+
+@pytest.mark.parametrize("args,rc", [
+    ((A, A, A, 1, 2, 4, 64, 2, 2, 128, 0, A, None), SHAPE),  # weights of fp16
+    ((A, A, A, 0, 1, 4, 64, 2, 2, 128, 0, A, None), SHAPE),  # weights' rows shorter than k
+    ((A, A, None, 0, 0, 4, 64, 2, 2, 128, 9, A, None), SHAPE), ((None, A, None, 0, 0, 4, 64, 2, 2, 128, 0, A, None), ARG),
+    ((A, A, None, 0, 0, 4, 64, 2, 2, 128, 0, None, None), ARG), ((A, A, None, 0, 0, 0, 64, 2, 2, 128, 0, None, None), 0),
+])
+def test_unpermute_refuses(built_lib, args, rc):
+    assert built_lib.xmoe_unpermute(*args) == rc
+
+
+@pytest.mark.parametrize("drows,dw,rc", [(None, A, ARG), (A, None, ARG), (2 * A, A, ARG)])
+def test_unpermute_backward_refuses(built_lib, drows, dw, rc):
+    # rows at 2 * A: drows may not be the same buffer
+    assert built_lib.xmoe_unpermute_backward(A, 2 * A, A, None, 0, 0, 4, 64, 2, 2, 128, 0, drows, dw, None) == rc
+
+
+@pytest.mark.parametrize("args,rc", [
+    ((A, 0, 4, 64, 32, None, 0, 0, 0, A, 64, A, 4, None), SHAPE),    # rows overlap
+    ((A, 0, 4, 64, 64, None, 0, 0, 0, A, 72, A, 4, None), SHAPE),    # code rows not at multiples of 16
+    ((A, 0, 4, 64, 64, None, 0, 0, 0, A, 64, A, 3, None), SHAPE),    # scales shorter than the rows
+    ((A, 0, 4, 64, 64, None, 0, 0, 0, A + 8, 64, A, 4, None), SHAPE),
+    ((A, 5, 4, 64, 64, None, 0, 0, 0, A, 64, A, 4, None), SHAPE), ((A, 0, -4, 64, 64, None, 0, 0, 0, A, 64, A, 4, None), ARG),
+    ((A, 0, 4, 64, 64, A, 2, 1, 128, A, 64, A, 128, None), SHAPE),   # plan's rows shorter than k
+    ((A, 0, 4, 64, 64, A, 2, 2, 128, A, 64, A, 124, None), SHAPE), ((A, 0, 4, 64, 64, A, 2, 2, -1, A, 64, A, 128, None), ARG),
+    ((None, 0, 0, 64, 64, None, 0, 0, 0, None, 64, None, 0, None), 0),
+])
+def test_quant_refuses(built_lib, args, rc):
+    assert built_lib.xmoe_fp8_quant(*args) == rc
+
+
+def test_glu_and_weight_quant_refuse(built_lib):
+    lib = built_lib
+    ok = (A, 0, 8, 64, 0, 1.0, 1.0, None, None, 0, A, 64, A, 8, None)
+
+    def glu(**kw):
+        names = "h dtype rows inter act alpha limit counts offsets mats q ldq scale lds stream".split()
+        return lib.xmoe_glu_fp8_quant(*{**dict(zip(names, ok)), **kw}.values())
+
+    assert glu(rows=-1) == ARG and glu(act=3) == SHAPE and glu(ldq=48) == SHAPE and glu(lds=4) == SHAPE
+    assert glu(counts=A) == ARG and glu(counts=A, offsets=A, mats=2000) == LIMIT and glu(h=None) == ARG
+    assert glu(rows=0, lds=0) == 0
+    assert lib.xmoe_glu_backward(A, A, 0, 8, 64, 0, 1.0, 1.0, None, None, 0, A, None) == ARG  # in place
+    assert lib.xmoe_glu_backward(A, A, 0, 8, 0, 0, 1.0, 1.0, None, None, 0, 2 * A, None) == SHAPE
+    assert lib.xmoe_fp8_quant_weight(A, 0, 1, 64, 64, A, 32, A, None) == SHAPE
+    assert lib.xmoe_fp8_quant_weight(A, 0, 1, 64, 64, None, 64, A, None) == ARG
+    assert lib.xmoe_fp8_quant_weight(A, 0, 0, 64, 64, None, 64, None, None) == 0
+
+
+def test_products_refuse(built_lib):
+    lib = built_lib
+    names = "x ldx xs lds w ldw wmat ws counts offsets mats rows used n k tr out odt ldo stream".split()
+    ok = dict(zip(names, (A, 128, A, 8, A, 128, 256 * 128, A, A, A, 2, 8, 0, 256, 128, 0, A, 0, 256, None)))
+
+    def grouped(**kw):
+        return lib.xmoe_fp8_grouped_gemm(*{**ok, **kw}.values())
+
+    assert grouped(ldx=112) == SHAPE and grouped(ldx=136) == SHAPE and grouped(ldw=120) == SHAPE and grouped(lds=4) == SHAPE
+    assert grouped(lds=10) == SHAPE and grouped(ldo=128) == SHAPE and grouped(wmat=128) == SHAPE
+    assert grouped(wmat=256 * 128 + 8) == SHAPE and grouped(odt=3) == SHAPE and grouped(n=0) == SHAPE and grouped(mats=0) == SHAPE
+    assert grouped(mats=2000) == LIMIT and grouped(rows=-1) == ARG and grouped(used=-1) == ARG and grouped(x=None) == ARG
+    assert grouped(counts=None) == ARG and grouped(xs=A + 4) == SHAPE and grouped(out=None) == ARG
+    assert grouped(tr=1) == SHAPE  # contracts over n = 256: x is too narrow
+    assert grouped(rows=0, lds=0) == 0
+    assert lib.xmoe_fp8_gemm(A, 120, A, 8, A, 128, A, 8, 256, 128, 0, A, 0, 256, None) == SHAPE
+    assert lib.xmoe_fp8_status(None, None) == ARG
+
+
+def test_python_refuses_what_it_cannot_do():
+    x = torch.zeros(4, 64)
+    plan = torch.zeros(4, 2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="num_rows or out"):
+        ops.permute(x, plan)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        ops.permute(x.clone().requires_grad_(), plan, out=torch.zeros(128, 64))
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        ops.unpermute(x.clone().requires_grad_(), plan, out=torch.zeros(4, 64))
+    with pytest.raises(RuntimeError, match="num_rows or out"):
+        fp8.quant(x, plan)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.route_pack(plan, plan.bfloat16(), 8)
+    with pytest.raises(NotImplementedError):  # no CPU kernel, no fallback
+        fp8.matmul(x.to(torch.float8_e4m3fn), torch.ones(4, 1), x.to(torch.float8_e4m3fn), torch.ones(1, 1))
+
+
+def test_layout_of_empty_rows():
+    codes, scale = fp8.empty_rows(5, 130, "cpu")
+    assert codes.shape == (5, 130) and codes.stride() == (144, 1) and codes.dtype == torch.float8_e4m3fn
+    assert scale.shape == (5, 2) and scale.stride() == (1, 8)
+
+
+def test_plain_rounding_is_the_formats():
+    """e4m3_round against torch's own conversion, on every value, every midpoint and its fp32 neighbours."""
+    v = P.e4m3_values()
+    mid = ((v[1:] + v[:-1]) / 2).float()
+    all_of = torch.cat([v.float(), mid, mid.nextafter(torch.tensor(1e9)), mid.nextafter(torch.tensor(0.0))])
+    all_of = torch.cat([all_of, -all_of])
+    assert torch.equal(P.e4m3_round(all_of.double()), all_of.to(torch.float8_e4m3fn).double())
+
+
+def test_ctypes_signatures_of_the_new_calls(built_lib):
+    for name in ("xmoe_permute", "xmoe_fp8_grouped_gemm", "xmoe_fp8_status"):
+        assert name in _lib.SIGNATURES and getattr(built_lib, name).restype is C.c_int

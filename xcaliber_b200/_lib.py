@@ -108,6 +108,17 @@ SIGNATURES = {
     "xmoe_repack_gptq": (C.c_int, [_P, _P, _I, _I, _I, _P]),
     "xmoe_repack_int4_kmajor": (C.c_int, [_P, _P, _SZ, _P]),
     "xmoe_fill_sigmoid_lut": (None, [_P]),
+    "xmoe_permute": (C.c_int, [_P, _P, _I, _I, _I, _I, _I, _I, _P, _P]),
+    "xmoe_unpermute": (C.c_int, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P]),
+    "xmoe_unpermute_backward": (C.c_int, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P]),
+    "xmoe_fp8_quant": (C.c_int, [_P, _I, _I, _I, _I, _P, _I, _I, _I, _P, _I, _P, _I, _P]),
+    "xmoe_fp8_quant_weight": (C.c_int, [_P, _I, _I, _I, _I, _P, _I, _P, _P]),
+    "xmoe_glu_fp8_quant": (C.c_int, [_P, _I, _I, _I, _I, _F, _F, _P, _P, _I, _P, _I, _P, _I, _P]),
+    "xmoe_glu_backward": (C.c_int, [_P, _P, _I, _I, _I, _I, _F, _F, _P, _P, _I, _P, _P]),
+    "xmoe_fp8_gemm": (C.c_int, [_P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _I, _I, _P]),
+    "xmoe_fp8_grouped_gemm": (C.c_int, [_P, _I, _P, _I, _P, _I, C.c_int64, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _I, _I,
+                                        _P]),
+    "xmoe_fp8_status": (C.c_int, [C.POINTER(C.c_uint32), _P]),
 }
 
 

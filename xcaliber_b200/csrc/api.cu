@@ -68,6 +68,24 @@ int make_tmap_kslabs(CUtensorMap* out, CUtensorMapDataType dt, int elem_bytes, c
     return r == CUDA_SUCCESS ? XMOE_OK : XMOE_ERR_CUDA;
 }
 
+// 8-bit codes: rows of `inner` bytes `ld` bytes apart (a multiple of 16; `inner` need not be one), the rows of matrix e
+// starting at byte e * mat_stride (mats > 0: a 3-D view [mats][rows][inner], so that a box never reaches into the next
+// matrix). Elements outside read as zero.
+int make_tmap_codes(CUtensorMap* out, const void* base, uint64_t inner, uint64_t rows, uint64_t mats, uint64_t ld,
+                    uint64_t mat_stride, uint32_t box_rows) {
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn) return XMOE_ERR_CUDA;
+    if ((reinterpret_cast<uintptr_t>(base) & 15u) || (ld & 15u) || (mat_stride & 15u)) return XMOE_ERR_SHAPE;
+    cuuint64_t dims[3] = {inner, rows, mats};
+    cuuint64_t strides[2] = {ld, mat_stride};
+    cuuint32_t box[3] = {128, box_rows, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, mats ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? XMOE_OK : XMOE_ERR_CUDA;
+}
+
 int num_sms() {  // of the current device
     static int n_dev[kMaxDevices] = {};
     const int dev = device_slot();
@@ -607,6 +625,64 @@ int forward_impl(const xmoe_config* cfg, const xmoe_weights* w, const void* x, c
     return rc;
 }
 
+// ---- operators around FP8 experts ---------------------------------------------------------------------------
+bool is_elem_type(int dtype) { return dtype == XMOE_BF16 || dtype == XMOE_FP16 || dtype == XMOE_FP32; }
+
+// Arguments that the three permutations share. Returns XMOE_OK with *empty set when there is nothing to do.
+int check_permute(const PermuteArgs& a, bool* empty) {
+    *empty = false;
+    if (a.N < 0 || a.k < 0 || a.num_rows < 0) return XMOE_ERR_ARG;
+    if (!is_elem_type(a.dtype) || (a.w && a.w_dtype != XMOE_BF16 && a.w_dtype != XMOE_FP32)) return XMOE_ERR_SHAPE;
+    if (a.H <= 0 || a.idx_stride < a.k || (a.w && a.w_stride < a.k)) return XMOE_ERR_SHAPE;
+    *empty = a.N == 0;
+    if (*empty) return XMOE_OK;
+    if (!a.x || (!a.topk_row && a.k) || (!a.rows && a.num_rows && a.k)) return XMOE_ERR_ARG;
+    return XMOE_OK;
+}
+
+// Token tile of a product: the smallest of 16 / 32 / 64 / 128 / 256 that holds an expert's rows on average.
+int fp8_token_tile(size_t rows, size_t mats) {
+    const size_t live = mats < rows ? mats : rows;
+    const size_t avg = live ? (rows + live - 1) / live : 0;
+    return avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : avg <= 128 ? 128 : 256;
+}
+
+int run_fp8_gemm(const void* x, int ldx, const float* x_scale, int lds, const void* w, int ldw, int64_t w_mat_stride,
+                 const float* w_scale, const int32_t* counts, const int32_t* offsets, int mats, int rows, int rows_in_use,
+                 int n, int k, bool transpose, void* out, int out_dtype, int ldo, cudaStream_t stream) {
+    if (rows < 0 || rows_in_use < 0) return XMOE_ERR_ARG;
+    if (n <= 0 || k <= 0 || mats <= 0 || !is_elem_type(out_dtype)) return XMOE_ERR_SHAPE;
+    if (mats > 1032) return XMOE_ERR_LIMIT;
+    const int contraction = transpose ? n : k, features = transpose ? k : n;
+    if (ldx < contraction || ldx % 16 || ldw < k || ldw % 16 || lds < rows || lds % 4 || ldo < features) return XMOE_ERR_SHAPE;
+    if (mats > 1 && (w_mat_stride < (int64_t)ldw * (n - 1) + k || w_mat_stride % 16)) return XMOE_ERR_SHAPE;
+    if (rows == 0) return XMOE_OK;
+    if (!x || !x_scale || !w || !w_scale || !out) return XMOE_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(x_scale) & 15u) return XMOE_ERR_SHAPE;
+    Fp8GemmArgs a;
+    memset(&a, 0, sizeof(a));
+    const int tile = fp8_token_tile((size_t)(rows_in_use && rows_in_use < rows ? rows_in_use : rows), (size_t)mats);
+    int rc = make_tmap_codes(&a.tm_w, w, (uint64_t)k, (uint64_t)n, (uint64_t)mats, (uint64_t)ldw,
+                             mats > 1 ? (uint64_t)w_mat_stride : (uint64_t)ldw * (uint64_t)n, 128);
+    if (rc) return rc;
+    rc = make_tmap_codes(&a.tm_x, x, (uint64_t)contraction, (uint64_t)rows, 0, (uint64_t)ldx, 0, (uint32_t)tile);
+    if (rc) return rc;
+    a.x_scale = x_scale;
+    a.w_scale = w_scale;
+    a.counts = counts;
+    a.offsets = offsets;
+    a.out = out;
+    a.rows = rows;
+    a.lds = lds;
+    a.ldo = ldo;
+    a.mats = mats;
+    a.out_features = features;
+    a.contraction = contraction;
+    a.out_dtype = out_dtype;
+    a.num_sms = num_sms();
+    return launch_fp8_gemm(a, tile, transpose, stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -1101,6 +1177,151 @@ int xmoe_repack_gptq(const void* qweight, void* out, int32_t num_mats, int32_t k
 int xmoe_repack_int4_kmajor(const void* w_in, void* out, size_t n_words, xmoe_stream_t stream) {
     if (!w_in || !out) return XMOE_ERR_ARG;
     return launch_repack_kmajor_int4(w_in, out, n_words, (cudaStream_t)stream);
+}
+
+int xmoe_permute(const void* x, const int32_t* topk_row, int32_t n, int32_t hidden, int32_t k, int32_t idx_stride,
+                 int32_t num_rows, int32_t dtype, void* rows, xmoe_stream_t stream) {
+    PermuteArgs a{x, rows, nullptr, topk_row, nullptr, nullptr, n, hidden, k, idx_stride, 0, num_rows, dtype, 0};
+    bool empty;
+    const int rc = check_permute(a, &empty);
+    if (rc || empty || num_rows == 0 || k == 0) return rc;
+    return launch_permute(a, (cudaStream_t)stream);
+}
+
+int xmoe_unpermute(const void* rows, const int32_t* topk_row, const void* w, int32_t w_dtype, int32_t w_stride, int32_t n,
+                   int32_t hidden, int32_t k, int32_t idx_stride, int32_t num_rows, int32_t dtype, void* y,
+                   xmoe_stream_t stream) {
+    PermuteArgs a{y, rows, nullptr, topk_row, w, nullptr, n, hidden, k, idx_stride, w_stride, num_rows, dtype, w_dtype};
+    bool empty;
+    const int rc = check_permute(a, &empty);
+    if (rc || empty) return rc;
+    return launch_unpermute(a, (cudaStream_t)stream);
+}
+
+int xmoe_unpermute_backward(const void* dy, const void* rows, const int32_t* topk_row, const void* w, int32_t w_dtype,
+                            int32_t w_stride, int32_t n, int32_t hidden, int32_t k, int32_t idx_stride, int32_t num_rows,
+                            int32_t dtype, void* drows, float* dw, xmoe_stream_t stream) {
+    PermuteArgs a{dy, rows, drows, topk_row, w, dw, n, hidden, k, idx_stride, w_stride, num_rows, dtype, w_dtype};
+    bool empty;
+    const int rc = check_permute(a, &empty);
+    if (rc || empty || k == 0) return rc;
+    if (!dw || (!drows && num_rows) || (drows && drows == rows)) return XMOE_ERR_ARG;
+    return launch_unpermute_backward(a, (cudaStream_t)stream);
+}
+
+int xmoe_fp8_quant(const void* x, int32_t dtype, int32_t rows, int32_t cols, int32_t ldx, const int32_t* topk_row, int32_t k,
+                   int32_t idx_stride, int32_t num_rows, void* q, int32_t ldq, float* scale, int32_t lds,
+                   xmoe_stream_t stream) {
+    if (rows < 0 || (topk_row && (k < 0 || num_rows < 0))) return XMOE_ERR_ARG;
+    if (!is_elem_type(dtype) || cols <= 0 || ldx < cols || ldq < cols || ldq % 16 || lds % 4) return XMOE_ERR_SHAPE;
+    if (topk_row ? (idx_stride < k || lds < num_rows) : lds < rows) return XMOE_ERR_SHAPE;
+    if (rows == 0 || (topk_row && (k == 0 || num_rows == 0))) return XMOE_OK;
+    if (!x || !q || !scale) return XMOE_ERR_ARG;
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(scale)) & 15u) return XMOE_ERR_SHAPE;
+    Fp8QuantArgs a;
+    memset(&a, 0, sizeof(a));
+    a.x = x;
+    a.q = (uint8_t*)q;
+    a.scale = scale;
+    a.topk_row = topk_row;
+    a.rows = rows;
+    a.cols = cols;
+    a.ldx = ldx;
+    a.ldq = ldq;
+    a.lds = lds;
+    a.k = k;
+    a.idx_stride = idx_stride;
+    a.num_rows = num_rows;
+    a.dtype = dtype;
+    return launch_fp8_quant(a, (cudaStream_t)stream);
+}
+
+int xmoe_fp8_quant_weight(const void* w, int32_t dtype, int32_t mats, int32_t n, int32_t k, void* q, int32_t ldq,
+                          float* scale, xmoe_stream_t stream) {
+    if (mats < 0) return XMOE_ERR_ARG;
+    if (!is_elem_type(dtype) || n <= 0 || k <= 0 || ldq < k || ldq % 16) return XMOE_ERR_SHAPE;
+    if (mats == 0) return XMOE_OK;
+    if (!w || !q || !scale) return XMOE_ERR_ARG;
+    return launch_fp8_quant_weight(w, dtype, mats, n, k, (uint8_t*)q, ldq, scale, (cudaStream_t)stream);
+}
+
+int xmoe_glu_fp8_quant(const void* h, int32_t dtype, int32_t rows, int32_t inter, int32_t activation, float alpha,
+                       float limit, const int32_t* counts, const int32_t* offsets, int32_t mats, void* q, int32_t ldq,
+                       float* scale, int32_t lds, xmoe_stream_t stream) {
+    if (rows < 0) return XMOE_ERR_ARG;
+    if (!is_elem_type(dtype) || inter <= 0 || activation < 0 || activation > 2 || ldq < inter || ldq % 16 || lds < rows || lds % 4)
+        return XMOE_ERR_SHAPE;
+    if (inter > 0x3fffffff || (counts && (!offsets || mats <= 0))) return XMOE_ERR_ARG;
+    if (counts && mats > 1032) return XMOE_ERR_LIMIT;
+    if (rows == 0) return XMOE_OK;
+    if (!h || !q || !scale) return XMOE_ERR_ARG;
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(scale)) & 15u) return XMOE_ERR_SHAPE;
+    Fp8QuantArgs a;
+    memset(&a, 0, sizeof(a));
+    a.x = h;
+    a.q = (uint8_t*)q;
+    a.scale = scale;
+    a.counts = counts;
+    a.offsets = offsets;
+    a.e_tot = mats;
+    a.rows = rows;
+    a.cols = inter;
+    a.ldx = 2 * inter;
+    a.ldq = ldq;
+    a.lds = lds;
+    a.dtype = dtype;
+    a.activation = activation;
+    a.alpha = alpha;
+    a.limit = limit;
+    return launch_glu_fp8_quant(a, (cudaStream_t)stream);
+}
+
+int xmoe_glu_backward(const void* da, const void* h, int32_t dtype, int32_t rows, int32_t inter, int32_t activation,
+                      float alpha, float limit, const int32_t* counts, const int32_t* offsets, int32_t mats, void* dh,
+                      xmoe_stream_t stream) {
+    if (rows < 0) return XMOE_ERR_ARG;
+    if (!is_elem_type(dtype) || inter <= 0 || activation < 0 || activation > 2) return XMOE_ERR_SHAPE;
+    if (inter > 0x3fffffff || (counts && (!offsets || mats <= 0))) return XMOE_ERR_ARG;
+    if (counts && mats > 1032) return XMOE_ERR_LIMIT;
+    if (rows == 0) return XMOE_OK;
+    if (!da || !h || !dh || dh == h) return XMOE_ERR_ARG;
+    Fp8QuantArgs a;
+    memset(&a, 0, sizeof(a));
+    a.x = h;
+    a.da = da;
+    a.dh = dh;
+    a.counts = counts;
+    a.offsets = offsets;
+    a.e_tot = mats;
+    a.rows = rows;
+    a.cols = inter;
+    a.ldx = 2 * inter;
+    a.dtype = dtype;
+    a.activation = activation;
+    a.alpha = alpha;
+    a.limit = limit;
+    return launch_glu_backward(a, (cudaStream_t)stream);
+}
+
+int xmoe_fp8_gemm(const void* x, int32_t ldx, const float* x_scale, int32_t lds, const void* w, int32_t ldw,
+                  const float* w_scale, int32_t rows, int32_t n, int32_t k, int32_t transpose, void* out, int32_t out_dtype,
+                  int32_t ldo, xmoe_stream_t stream) {
+    return run_fp8_gemm(x, ldx, x_scale, lds, w, ldw, 0, w_scale, nullptr, nullptr, 1, rows, rows, n, k, transpose != 0, out,
+                        out_dtype, ldo, (cudaStream_t)stream);
+}
+
+int xmoe_fp8_grouped_gemm(const void* x, int32_t ldx, const float* x_scale, int32_t lds, const void* w, int32_t ldw,
+                          int64_t w_mat_stride, const float* w_scale, const int32_t* counts, const int32_t* offsets,
+                          int32_t mats, int32_t rows, int32_t rows_in_use, int32_t n, int32_t k, int32_t transpose,
+                          void* out, int32_t out_dtype, int32_t ldo, xmoe_stream_t stream) {
+    if (rows > 0 && (!counts || !offsets)) return XMOE_ERR_ARG;
+    return run_fp8_gemm(x, ldx, x_scale, lds, w, ldw, w_mat_stride, w_scale, counts, offsets, mats, rows, rows_in_use, n, k,
+                        transpose != 0, out, out_dtype, ldo, (cudaStream_t)stream);
+}
+
+int xmoe_fp8_status(uint32_t* host_out, xmoe_stream_t stream) {
+    if (!host_out) return XMOE_ERR_ARG;
+    return fp8_read_status(host_out, (cudaStream_t)stream);
 }
 
 void xmoe_fill_sigmoid_lut(float* host_out) {

@@ -166,6 +166,56 @@ struct ActTopkArgs {
     int max_rows;  // grid bound (R_cap)
 };
 
+// Tokens sorted by expert and back (permute.cu). x: the token side (input of permute; OUTPUT of unpermute; dy of the
+// backward), [N, H]; rows / drows [num_rows, H]; element types XMOE_BF16 / _FP16 / _FP32.
+struct PermuteArgs {
+    const void* x;
+    const void* rows;
+    void* drows;
+    const int32_t* topk_row;  // [N, idx_stride]
+    const void* w;            // bf16 or fp32 [N, w_stride], or null
+    float* dw;                // [N, k]
+    int N, H, k, idx_stride, w_stride, num_rows;
+    int dtype, w_dtype;
+};
+int launch_permute(const PermuteArgs& a, cudaStream_t stream);
+int launch_unpermute(const PermuteArgs& a, cudaStream_t stream);
+int launch_unpermute_backward(const PermuteArgs& a, cudaStream_t stream);
+
+// Quantisation to e4m3 with one scale per 128 values (fp8_quant.cu).
+struct Fp8QuantArgs {
+    const void* x;            // [rows, ldx], element type dtype; GLU: [rows, 2 * cols] = gate | up
+    uint8_t* q;               // [out rows, ldq]
+    float* scale;             // [ceil(cols / 128), lds]
+    const int32_t* topk_row;  // plain rows only: where each of the k slots of a row goes, or null (row r -> row r)
+    const int32_t* counts;    // GLU only: live rows per expert, or null (all rows are live)
+    const int32_t* offsets;
+    const void* da;           // GLU backward: gradient of the activation [rows, cols]
+    void* dh;                 // GLU backward: [rows, 2 * cols]
+    int rows, cols, ldx, ldq, lds, k, idx_stride, num_rows, e_tot;
+    int dtype, activation;
+    float alpha, limit;
+};
+int launch_fp8_quant(const Fp8QuantArgs& a, cudaStream_t stream);
+int launch_fp8_quant_weight(const void* w, int dtype, int mats, int n, int k, uint8_t* q, int ldq, float* scale,
+                            cudaStream_t stream);
+int launch_glu_fp8_quant(const Fp8QuantArgs& a, cudaStream_t stream);
+int launch_glu_backward(const Fp8QuantArgs& a, cudaStream_t stream);
+
+// Block-scaled e4m3 product (fp8_gemm.cu). Output features are the weight's rows (or, transposed, its columns).
+struct Fp8GemmArgs {
+    CUtensorMap tm_w;        // u8 [mats][n][k] of the weight, box 128 x 128, 128-byte swizzle
+    CUtensorMap tm_x;        // u8 [rows][contraction] of the tokens, box 128 x token tile, 128-byte swizzle
+    const float* x_scale;    // [contraction blocks, lds]
+    const float* w_scale;    // [mats, ceil(n / 128), ceil(k / 128)]
+    const int32_t* counts;   // [mats], or null: one matrix, all rows
+    const int32_t* offsets;  // [mats + 1]
+    void* out;               // [rows, ldo]
+    int rows, lds, ldo, mats, out_features, contraction, out_dtype, num_sms;
+};
+int launch_fp8_gemm(const Fp8GemmArgs& a, int token_tile, bool transpose, cudaStream_t stream);
+int fp8_read_status(uint32_t* host_out, cudaStream_t stream);
+
 int launch_router_topk(const RouterArgs& a, cudaStream_t stream);
 int route_pack_chunks(int N);
 int launch_route_pack(const PackArgs& a, cudaStream_t stream);

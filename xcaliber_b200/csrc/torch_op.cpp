@@ -1,5 +1,6 @@
 // PyTorch custom-op registration of the fused MoE operator: `torch.ops.xmoe_b200.{forward, repack_gptq,
-// prep_nvfp4_sf, build_info}`. This is the vLLM-facing counterpart of the reference's torch extension module
+// prep_nvfp4_sf, build_info}`, and of the operators around FP8 experts (permute .. fp8_grouped_matmul below: they write
+// into tensors of the caller, ops.py and fp8.py allocate). This is the vLLM-facing counterpart of the reference's torch extension module
 // (xFused-XXXX-Kernels/xMoE/xW4A16/sm75/xR64/vllm/csrc/xr64_abs_bridge.cu:61-242: `_C.forward`,
 // `_C.repack_gptq`, `_C.build_info`), registered through TORCH_LIBRARY instead of pybind11 so that the
 // dispatcher, torch.compile (through the Meta kernels below) and CUDA-graph capture see a real operator
@@ -156,6 +157,295 @@ at::Tensor prep_nvfp4_sf_meta(const at::Tensor& scale, int64_t rows_per_mat) {
 
 std::string build_info() { return xmoe_build_info(); }
 
+// ---- operators around FP8 experts: each checks its tensors, makes their device current and enqueues on its stream ----
+int32_t elem_type(const at::Tensor& t, const char* name) {
+    switch (t.scalar_type()) {
+        case at::kBFloat16: return XMOE_BF16;
+        case at::kHalf: return XMOE_FP16;
+        case at::kFloat: return XMOE_FP32;
+        default: TORCH_CHECK(false, name, " must be bf16, fp16 or fp32");
+    }
+}
+void check_matrix(const at::Tensor& t, const at::Tensor& like, const char* name) {
+    check_cuda_contig(t, like, name);
+    TORCH_CHECK(t.dim() == 2, name, " must be a matrix");
+}
+int32_t i32(int64_t v, const char* name) {
+    TORCH_CHECK(v >= 0 && v <= 0x7fffffff, name, " is beyond 32 bits");
+    return (int32_t)v;
+}
+void check_rc(int rc, const char* what) { TORCH_CHECK(rc == XMOE_OK, what, ": ", xmoe_status_string(rc)); }
+xmoe_stream_t stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+// topk_row i32 [N, k], rows of any stride
+int32_t check_plan(const at::Tensor& plan, int64_t n, const at::Tensor& like) {
+    TORCH_CHECK(plan.is_cuda() && plan.device() == like.device() && plan.scalar_type() == at::kInt && plan.dim() == 2 &&
+                    plan.size(0) == n && (plan.size(1) <= 1 || plan.stride(1) == 1),
+                "topk_row must be an int32 CUDA tensor [N, k] with contiguous rows, on the device of the other tensors");
+    return i32(n > 1 ? plan.stride(0) : plan.size(1), "topk_row's stride");
+}
+struct SlotWeights { const void* p = nullptr; int32_t type = 0, stride = 0; };
+SlotWeights check_weights(const c10::optional<at::Tensor>& w, const at::Tensor& plan) {
+    SlotWeights r;
+    if (!w.has_value() || !w->defined()) return r;
+    TORCH_CHECK(w->is_cuda() && w->device() == plan.device() && w->sizes() == plan.sizes() &&
+                    (w->size(1) <= 1 || w->stride(1) == 1) &&
+                    (w->scalar_type() == at::kBFloat16 || w->scalar_type() == at::kFloat),
+                "weights must be a bf16 or fp32 CUDA tensor of topk_row's shape with contiguous rows");
+    r.p = w->data_ptr();
+    r.type = elem_type(*w, "weights");
+    r.stride = i32(w->size(0) > 1 ? w->stride(0) : w->size(1), "the weights' stride");
+    return r;
+}
+
+void permute_cuda(const at::Tensor& x, const at::Tensor& topk_row, at::Tensor& rows) {
+    check_matrix(x, x, "x");
+    check_matrix(rows, x, "rows");
+    const int32_t ld = check_plan(topk_row, x.size(0), x);
+    TORCH_CHECK(rows.scalar_type() == x.scalar_type() && rows.size(1) == x.size(1), "rows must have x's type and width");
+    if (x.numel() == 0 || rows.numel() == 0 || topk_row.numel() == 0) return;
+    c10::cuda::CUDAGuard guard(x.device());
+    check_rc(xmoe_permute(x.data_ptr(), topk_row.data_ptr<int32_t>(), i32(x.size(0), "N"), i32(x.size(1), "hidden"),
+                          i32(topk_row.size(1), "k"), ld, i32(rows.size(0), "rows"), elem_type(x, "x"), rows.data_ptr(),
+                          stream_of(x)),
+             "xmoe_permute");
+}
+
+void unpermute_cuda(const at::Tensor& rows, const at::Tensor& topk_row, const c10::optional<at::Tensor>& weights,
+                    at::Tensor& y) {
+    check_matrix(rows, rows, "rows");
+    check_matrix(y, rows, "y");
+    const int32_t ld = check_plan(topk_row, y.size(0), rows);
+    const SlotWeights w = check_weights(weights, topk_row);
+    TORCH_CHECK(rows.scalar_type() == y.scalar_type() && rows.size(1) == y.size(1), "y must have the rows' type and width");
+    if (y.numel() == 0) return;
+    c10::cuda::CUDAGuard guard(rows.device());
+    check_rc(xmoe_unpermute(rows.data_ptr(), topk_row.data_ptr<int32_t>(), w.p, w.type, w.stride, i32(y.size(0), "N"),
+                            i32(y.size(1), "hidden"), i32(topk_row.size(1), "k"), ld, i32(rows.size(0), "rows"),
+                            elem_type(rows, "rows"), y.data_ptr(), stream_of(rows)),
+             "xmoe_unpermute");
+}
+
+void unpermute_backward_cuda(const at::Tensor& dy, const at::Tensor& rows, const at::Tensor& topk_row,
+                             const c10::optional<at::Tensor>& weights, at::Tensor& drows, at::Tensor& dw) {
+    check_matrix(dy, dy, "dy");
+    check_matrix(rows, dy, "rows");
+    check_matrix(drows, dy, "drows");
+    check_matrix(dw, dy, "dw");
+    const int32_t ld = check_plan(topk_row, dy.size(0), dy);
+    const SlotWeights w = check_weights(weights, topk_row);
+    TORCH_CHECK(rows.scalar_type() == dy.scalar_type() && rows.size(1) == dy.size(1), "rows must have dy's type and width");
+    TORCH_CHECK(drows.scalar_type() == dy.scalar_type() && drows.sizes() == rows.sizes(), "drows must be like rows");
+    TORCH_CHECK(dw.scalar_type() == at::kFloat && dw.sizes() == topk_row.sizes(), "dw must be fp32 [N, k]");
+    if (dw.numel() == 0) return;
+    if (dy.size(1) == 0) {
+        dw.zero_();
+        return;
+    }
+    c10::cuda::CUDAGuard guard(dy.device());
+    check_rc(xmoe_unpermute_backward(dy.data_ptr(), rows.data_ptr(), topk_row.data_ptr<int32_t>(), w.p, w.type, w.stride,
+                                     i32(dy.size(0), "N"), i32(dy.size(1), "hidden"), i32(topk_row.size(1), "k"), ld,
+                                     i32(rows.size(0), "rows"), elem_type(dy, "dy"), drows.data_ptr(), dw.data_ptr<float>(),
+                                     stream_of(dy)),
+             "xmoe_unpermute_backward");
+}
+
+// Codes [rows, cols] whose rows start at multiples of 16 bytes; returns the distance of two rows.
+int32_t check_codes(const at::Tensor& q, const at::Tensor& like, const char* name) {
+    const int64_t d = q.dim(), cols = q.size(d - 1), rows = q.size(d - 2);
+    TORCH_CHECK(q.is_cuda() && q.device() == like.device() && q.scalar_type() == at::kFloat8_e4m3fn, name,
+                " must be a float8_e4m3fn CUDA tensor on the device of the other tensors");
+    TORCH_CHECK((cols <= 1 || q.stride(d - 1) == 1) && (rows <= 1 || (q.stride(d - 2) % 16 == 0 && q.stride(d - 2) >= cols)) &&
+                    (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15u) == 0,
+                name, "'s rows must be contiguous and start at multiples of 16 bytes (as fp8.quant lays them out)");
+    return i32(rows > 1 ? q.stride(d - 2) : (cols + 15) / 16 * 16, "the codes' row stride");
+}
+// Scales [rows, blocks] laid out block-major (stride (1, ld), ld a multiple of 4); returns ld, or -1 for another layout.
+int64_t scale_ld(const at::Tensor& s) {
+    const int64_t rows = s.size(0), blocks = s.size(1);
+    if (reinterpret_cast<uintptr_t>(s.data_ptr()) & 15u) return -1;
+    if (rows > 1 && s.stride(0) != 1) return -1;
+    // each block's row is read to a multiple of 4: the last one's end must still belong to the storage
+    const int64_t up = (rows + 3) / 4 * 4, ld = blocks <= 1 ? up : s.stride(1);
+    if (ld % 4 || ld < rows) return -1;
+    const int64_t end = s.storage_offset() + (blocks - 1) * ld + up;
+    return end * 4 <= (int64_t)s.storage().nbytes() ? ld : -1;
+}
+at::Tensor block_major(const at::Tensor& s) {
+    at::Tensor room = at::empty({s.size(1), (s.size(0) + 3) / 4 * 4}, s.options());
+    at::Tensor t = room.narrow(1, 0, s.size(0)).t();
+    t.copy_(s);
+    return room;
+}
+int64_t blocks_of(int64_t cols) { return (cols + 127) / 128; }
+
+int32_t check_scale_out(const at::Tensor& s, int64_t rows, int64_t cols, const at::Tensor& like) {
+    TORCH_CHECK(s.is_cuda() && s.device() == like.device() && s.scalar_type() == at::kFloat && s.dim() == 2 &&
+                    s.size(0) == rows && s.size(1) == blocks_of(cols),
+                "scale must be fp32 [rows, ceil(cols / 128)]");
+    const int64_t ld = scale_ld(s);
+    TORCH_CHECK(ld >= 0, "scale must be laid out block-major: strides (1, multiple of 4), 16-byte aligned (as fp8.quant lays it out)");
+    return i32(ld, "the scales' stride");
+}
+
+void fp8_quant_cuda(const at::Tensor& x, const c10::optional<at::Tensor>& topk_row, at::Tensor& q, at::Tensor& scale) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(1) > 0 && (x.size(1) == 1 || x.stride(1) == 1) &&
+                    (x.size(0) <= 1 || x.stride(0) >= x.size(1)),
+                "x must be a CUDA matrix with contiguous rows");
+    const bool sorted = topk_row.has_value() && topk_row->defined();
+    TORCH_CHECK(q.dim() == 2 && q.size(1) == x.size(1) && (sorted || q.size(0) == x.size(0)), "codes must be [rows, cols] like x");
+    const int32_t ldq = check_codes(q, x, "codes");
+    const int32_t lds = check_scale_out(scale, q.size(0), x.size(1), x);
+    const int32_t ldp = sorted ? check_plan(*topk_row, x.size(0), x) : 0;
+    if (x.numel() == 0 || q.numel() == 0 || (sorted && topk_row->numel() == 0)) return;
+    c10::cuda::CUDAGuard guard(x.device());
+    check_rc(xmoe_fp8_quant(x.data_ptr(), elem_type(x, "x"), i32(x.size(0), "rows"), i32(x.size(1), "cols"),
+                            i32(x.size(0) > 1 ? x.stride(0) : x.size(1), "x's stride"),
+                            sorted ? topk_row->data_ptr<int32_t>() : nullptr, sorted ? i32(topk_row->size(1), "k") : 0, ldp,
+                            i32(q.size(0), "rows"), q.data_ptr(), ldq, scale.data_ptr<float>(), lds, stream_of(x)),
+             "xmoe_fp8_quant");
+}
+
+void fp8_quant_weight_cuda(const at::Tensor& w, at::Tensor& q, at::Tensor& scale) {
+    check_cuda_contig(w, w, "w");
+    check_cuda_contig(scale, w, "scale");
+    TORCH_CHECK(w.dim() == 3 && w.size(1) > 0 && w.size(2) > 0 && q.sizes() == w.sizes(), "w and codes must be [mats, n, k]");
+    const int32_t ldq = check_codes(q, w, "codes");
+    TORCH_CHECK(w.size(0) <= 1 || q.stride(0) == (int64_t)ldq * w.size(1), "the codes' matrices must follow one another");
+    TORCH_CHECK(scale.scalar_type() == at::kFloat && scale.dim() == 3 && scale.size(0) == w.size(0) &&
+                    scale.size(1) == blocks_of(w.size(1)) && scale.size(2) == blocks_of(w.size(2)),
+                "scale must be fp32 [mats, ceil(n / 128), ceil(k / 128)]");
+    if (w.numel() == 0) return;
+    c10::cuda::CUDAGuard guard(w.device());
+    check_rc(xmoe_fp8_quant_weight(w.data_ptr(), elem_type(w, "w"), i32(w.size(0), "mats"), i32(w.size(1), "n"),
+                                   i32(w.size(2), "k"), q.data_ptr(), ldq, scale.data_ptr<float>(), stream_of(w)),
+             "xmoe_fp8_quant_weight");
+}
+
+struct Segments { const int32_t* counts = nullptr; const int32_t* offsets = nullptr; int32_t mats = 0; };
+Segments check_segments(const c10::optional<at::Tensor>& counts, const c10::optional<at::Tensor>& offsets, const at::Tensor& like) {
+    Segments g;
+    const bool have = counts.has_value() && counts->defined();
+    TORCH_CHECK(have == (offsets.has_value() && offsets->defined()), "counts and offsets come together");
+    if (!have) return g;
+    for (const at::Tensor* t : {&*counts, &*offsets}) {
+        check_cuda_contig(*t, like, "counts / offsets");
+        TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 1, "counts and offsets must be int32 vectors");
+    }
+    TORCH_CHECK(counts->size(0) > 0 && offsets->size(0) >= counts->size(0), "offsets must have an entry for every expert");
+    g.counts = counts->data_ptr<int32_t>();
+    g.offsets = offsets->data_ptr<int32_t>();
+    g.mats = i32(counts->size(0), "experts");
+    return g;
+}
+
+void glu_fp8_quant_cuda(const at::Tensor& h, int64_t activation, double alpha, double limit,
+                        const c10::optional<at::Tensor>& counts, const c10::optional<at::Tensor>& offsets, at::Tensor& q,
+                        at::Tensor& scale) {
+    check_matrix(h, h, "h");
+    TORCH_CHECK(h.size(1) > 0 && h.size(1) % 2 == 0, "h must be [rows, 2 * inter] (gate | up)");
+    TORCH_CHECK(q.dim() == 2 && q.size(0) == h.size(0) && q.size(1) == h.size(1) / 2, "codes must be [rows, inter]");
+    const int32_t ldq = check_codes(q, h, "codes");
+    const int32_t lds = check_scale_out(scale, q.size(0), q.size(1), h);
+    const Segments g = check_segments(counts, offsets, h);
+    if (h.numel() == 0) return;
+    c10::cuda::CUDAGuard guard(h.device());
+    check_rc(xmoe_glu_fp8_quant(h.data_ptr(), elem_type(h, "h"), i32(h.size(0), "rows"), i32(h.size(1) / 2, "inter"),
+                                (int32_t)activation, (float)alpha, (float)limit, g.counts, g.offsets, g.mats, q.data_ptr(), ldq,
+                                scale.data_ptr<float>(), lds, stream_of(h)),
+             "xmoe_glu_fp8_quant");
+}
+
+void glu_backward_cuda(const at::Tensor& da, const at::Tensor& h, int64_t activation, double alpha, double limit,
+                       const c10::optional<at::Tensor>& counts, const c10::optional<at::Tensor>& offsets, at::Tensor& dh) {
+    check_matrix(h, h, "h");
+    check_matrix(da, h, "da");
+    check_matrix(dh, h, "dh");
+    TORCH_CHECK(h.size(1) > 0 && h.size(1) % 2 == 0, "h must be [rows, 2 * inter] (gate | up)");
+    TORCH_CHECK(da.scalar_type() == h.scalar_type() && da.size(0) == h.size(0) && da.size(1) == h.size(1) / 2,
+                "da must be [rows, inter] of h's type");
+    TORCH_CHECK(dh.scalar_type() == h.scalar_type() && dh.sizes() == h.sizes(), "dh must be like h");
+    const Segments g = check_segments(counts, offsets, h);
+    if (h.numel() == 0) return;
+    c10::cuda::CUDAGuard guard(h.device());
+    check_rc(xmoe_glu_backward(da.data_ptr(), h.data_ptr(), elem_type(h, "h"), i32(h.size(0), "rows"), i32(h.size(1) / 2, "inter"),
+                               (int32_t)activation, (float)alpha, (float)limit, g.counts, g.offsets, g.mats, dh.data_ptr(),
+                               stream_of(h)),
+             "xmoe_glu_backward");
+}
+
+// One product, grouped (counts given, w [mats, n, k]) or not (w [n, k]).
+void fp8_product(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w, const at::Tensor& w_scale,
+                 const Segments* g, bool transpose, int64_t rows_in_use, at::Tensor& out) {
+    TORCH_CHECK(x.dim() == 2 && w.dim() == (g ? 3 : 2), g ? "x must be a matrix and w [experts, n, k]" : "x and w must be matrices");
+    const int64_t n = w.size(w.dim() - 2), k = w.size(w.dim() - 1), rows = x.size(0);
+    const int64_t in = transpose ? n : k, features = transpose ? k : n;
+    TORCH_CHECK(n > 0 && k > 0, "w must not be empty");
+    const int32_t ldx = check_codes(x, x, "x");
+    const int32_t ldw = check_codes(w, x, "w");
+    // numbers go through std::to_string: a compiler whose libstdc++ is linked in statically has stream facets of its own,
+    // and an integer written to a stream that torch made then looks one up that is not there
+    TORCH_CHECK(x.size(1) == in, "x has ", std::to_string(x.size(1)), " columns, the product contracts over ", std::to_string(in));
+    TORCH_CHECK(x_scale.is_cuda() && x_scale.device() == x.device() && x_scale.scalar_type() == at::kFloat && x_scale.dim() == 2 &&
+                    x_scale.size(0) == rows && x_scale.size(1) == blocks_of(in),
+                "x_scale must be fp32 [rows, ceil(columns / 128)]");
+    check_cuda_contig(w_scale, x, "w_scale");
+    TORCH_CHECK(w_scale.scalar_type() == at::kFloat && w_scale.dim() == w.dim() && w_scale.size(-2) == blocks_of(n) &&
+                    w_scale.size(-1) == blocks_of(k) && (!g || w_scale.size(0) == w.size(0)),
+                "w_scale must be fp32 [.., ceil(n / 128), ceil(k / 128)]");
+    check_matrix(out, x, "out");
+    TORCH_CHECK(out.size(0) == rows && out.size(1) == features, "out must be [rows, ", std::to_string(features), "]");
+    const int32_t out_type = elem_type(out, "out");
+    if (g) {
+        TORCH_CHECK(g->counts && g->mats == w.size(0), "counts must have an entry for every expert of w");
+        TORCH_CHECK(w.size(0) == 1 || w.stride(0) % 16 == 0, "w's matrices must start at multiples of 16 bytes");
+    }
+    TORCH_CHECK(rows_in_use >= 0, "rows_in_use must not be negative");
+    if (rows == 0) return;
+    c10::cuda::CUDAGuard guard(x.device());
+    int64_t lds = scale_ld(x_scale);
+    at::Tensor relaid;
+    if (lds < 0) {
+        relaid = block_major(x_scale);
+        lds = relaid.size(1);
+    }
+    const float* xs = lds >= 0 && relaid.defined() ? relaid.data_ptr<float>() : x_scale.data_ptr<float>();
+    const int rc =
+        g ? xmoe_fp8_grouped_gemm(x.data_ptr(), ldx, xs, i32(lds, "the scales' stride"), w.data_ptr(), ldw,
+                                  w.size(0) > 1 ? w.stride(0) : 0, w_scale.data_ptr<float>(), g->counts, g->offsets, g->mats,
+                                  i32(rows, "rows"), i32(rows_in_use, "rows_in_use"), i32(n, "n"), i32(k, "k"), transpose,
+                                  out.data_ptr(), out_type, i32(features, "features"), stream_of(x))
+          : xmoe_fp8_gemm(x.data_ptr(), ldx, xs, i32(lds, "the scales' stride"), w.data_ptr(), ldw, w_scale.data_ptr<float>(),
+                          i32(rows, "rows"), i32(n, "n"), i32(k, "k"), transpose, out.data_ptr(), out_type,
+                          i32(features, "features"), stream_of(x));
+    check_rc(rc, g ? "xmoe_fp8_grouped_gemm" : "xmoe_fp8_gemm");
+}
+void fp8_matmul_cuda(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w, const at::Tensor& w_scale,
+                     bool transpose, at::Tensor& out) {
+    fp8_product(x, x_scale, w, w_scale, nullptr, transpose, 0, out);
+}
+void fp8_grouped_matmul_cuda(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w, const at::Tensor& w_scale,
+                             const at::Tensor& counts, const at::Tensor& offsets, bool transpose, int64_t rows_in_use,
+                             at::Tensor& out) {
+    const Segments g = check_segments(counts, offsets, x);
+    fp8_product(x, x_scale, w, w_scale, &g, transpose, rows_in_use, out);
+}
+
+// Fake tensors: every result is a tensor of the caller, so there is nothing to shape.
+void permute_meta(const at::Tensor&, const at::Tensor&, at::Tensor&) {}
+void unpermute_meta(const at::Tensor&, const at::Tensor&, const c10::optional<at::Tensor>&, at::Tensor&) {}
+void unpermute_backward_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const c10::optional<at::Tensor>&,
+                             at::Tensor&, at::Tensor&) {}
+void fp8_quant_meta(const at::Tensor&, const c10::optional<at::Tensor>&, at::Tensor&, at::Tensor&) {}
+void fp8_quant_weight_meta(const at::Tensor&, at::Tensor&, at::Tensor&) {}
+void glu_fp8_quant_meta(const at::Tensor&, int64_t, double, double, const c10::optional<at::Tensor>&,
+                        const c10::optional<at::Tensor>&, at::Tensor&, at::Tensor&) {}
+void glu_backward_meta(const at::Tensor&, const at::Tensor&, int64_t, double, double, const c10::optional<at::Tensor>&,
+                       const c10::optional<at::Tensor>&, at::Tensor&) {}
+void fp8_matmul_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, bool, at::Tensor&) {}
+void fp8_grouped_matmul_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                             const at::Tensor&, bool, int64_t, at::Tensor&) {}
+
 }  // namespace
 
 TORCH_LIBRARY(xmoe_b200, m) {
@@ -166,16 +456,51 @@ TORCH_LIBRARY(xmoe_b200, m) {
     m.def("repack_gptq(Tensor qweight) -> Tensor");
     m.def("prep_nvfp4_sf(Tensor scale_e4m3, int rows_per_mat) -> Tensor");
     m.def("build_info() -> str", &build_info);
+    m.def("permute(Tensor x, Tensor topk_row, Tensor(a!) rows) -> ()");
+    m.def("unpermute(Tensor rows, Tensor topk_row, Tensor? weights, Tensor(a!) y) -> ()");
+    m.def(
+        "unpermute_backward(Tensor dy, Tensor rows, Tensor topk_row, Tensor? weights, Tensor(a!) drows, Tensor(b!) dw) "
+        "-> ()");
+    m.def("fp8_quant(Tensor x, Tensor? topk_row, Tensor(a!) codes, Tensor(b!) scale) -> ()");
+    m.def("fp8_quant_weight(Tensor w, Tensor(a!) codes, Tensor(b!) scale) -> ()");
+    m.def(
+        "glu_fp8_quant(Tensor h, int activation, float alpha, float limit, Tensor? counts, Tensor? offsets, Tensor(a!) "
+        "codes, Tensor(b!) scale) -> ()");
+    m.def(
+        "glu_backward(Tensor da, Tensor h, int activation, float alpha, float limit, Tensor? counts, Tensor? offsets, "
+        "Tensor(a!) dh) -> ()");
+    m.def("fp8_matmul(Tensor x, Tensor x_scale, Tensor w, Tensor w_scale, bool transpose, Tensor(a!) out) -> ()");
+    m.def(
+        "fp8_grouped_matmul(Tensor x, Tensor x_scale, Tensor w, Tensor w_scale, Tensor counts, Tensor offsets, bool "
+        "transpose, int rows_in_use, Tensor(a!) out) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(xmoe_b200, CUDA, m) {
     m.impl("forward", &forward_cuda);
     m.impl("repack_gptq", &repack_gptq_cuda);
     m.impl("prep_nvfp4_sf", &prep_nvfp4_sf_cuda);
+    m.impl("permute", &permute_cuda);
+    m.impl("unpermute", &unpermute_cuda);
+    m.impl("unpermute_backward", &unpermute_backward_cuda);
+    m.impl("fp8_quant", &fp8_quant_cuda);
+    m.impl("fp8_quant_weight", &fp8_quant_weight_cuda);
+    m.impl("glu_fp8_quant", &glu_fp8_quant_cuda);
+    m.impl("glu_backward", &glu_backward_cuda);
+    m.impl("fp8_matmul", &fp8_matmul_cuda);
+    m.impl("fp8_grouped_matmul", &fp8_grouped_matmul_cuda);
 }
 
 TORCH_LIBRARY_IMPL(xmoe_b200, Meta, m) {
     m.impl("forward", &forward_meta);
     m.impl("repack_gptq", &repack_gptq_meta);
     m.impl("prep_nvfp4_sf", &prep_nvfp4_sf_meta);
+    m.impl("permute", &permute_meta);
+    m.impl("unpermute", &unpermute_meta);
+    m.impl("unpermute_backward", &unpermute_backward_meta);
+    m.impl("fp8_quant", &fp8_quant_meta);
+    m.impl("fp8_quant_weight", &fp8_quant_weight_meta);
+    m.impl("glu_fp8_quant", &glu_fp8_quant_meta);
+    m.impl("glu_backward", &glu_backward_meta);
+    m.impl("fp8_matmul", &fp8_matmul_meta);
+    m.impl("fp8_grouped_matmul", &fp8_grouped_matmul_meta);
 }

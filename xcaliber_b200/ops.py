@@ -10,7 +10,7 @@ import dataclasses
 
 import torch
 
-from . import _lib
+from . import _lib, torch_ops
 from ._lib import XMoEConfig, XMoEWeights, XMoEWorkspaceView, check
 from .synth import MoEShape
 
@@ -341,6 +341,134 @@ def combine(rows: torch.Tensor, topk_row: torch.Tensor, out: torch.Tensor | None
         check(_lib.lib().xmoe_combine(rows.data_ptr(), topk_row.data_ptr(), n, h, k, k, y.data_ptr(), _stream()),
               "xmoe_combine")
     return y
+
+
+# ---------------------------------------------------------------------------------------
+# tokens sorted by expert and back, for experts of any format
+# ---------------------------------------------------------------------------------------
+@dataclasses.dataclass
+class Routes:
+    """What route_pack makes of a batch's routing: where every slot's row is, and every expert's segment of rows."""
+
+    topk_row: torch.Tensor    # i32 [N, k_eff]: row of slot s of token t, -1 = none
+    topk_w: torch.Tensor      # bf16 [N, k_eff]; shared experts have weight 1
+    counts: torch.Tensor      # i32 [E_tot] rows per expert
+    offsets: torch.Tensor     # i32 [E_tot + 1] first row of every expert, multiples of 128
+    row_token: torch.Tensor   # i32 [num_rows] token of every live row
+    status: torch.Tensor      # i32 [4]; word 0 is 0x600 when an expert id lay outside [0, E)
+    num_rows: int             # rows a buffer needs: N * k_eff and up to 127 unused rows per expert
+    rows_in_use: int          # N * k_eff, an upper bound of the live rows
+
+
+def route_pack(topk_idx: torch.Tensor, topk_w: torch.Tensor, num_experts: int, num_shared: int = 0) -> Routes:
+    """The layer's permutation stage alone, for experts outside the fused layer: topk_idx int32 [N, k] (-1: a slot without
+    an expert) and topk_w bf16 [N, k], as router_topk returns them. Shared experts are appended as slots of every token."""
+    if topk_idx.dim() != 2 or topk_idx.dtype != torch.int32 or not topk_idx.is_cuda:
+        raise RuntimeError("topk_idx must be an int32 CUDA tensor [N, k]")
+    if topk_w.shape != topk_idx.shape or topk_w.dtype != torch.bfloat16 or topk_w.device != topk_idx.device:
+        raise RuntimeError("topk_w must be a bf16 tensor of topk_idx's shape")
+    n, k = topk_idx.shape
+    ke, et = k + num_shared, num_experts + num_shared
+    if not 0 < et <= 1032 or ke > 32:
+        raise RuntimeError("route_pack takes up to 1032 experts and 32 slots per token")
+    rows = -(-(n * ke + min(et, n * ke) * 127) // 128) * 128
+    dev = topk_idx.device
+    with torch.cuda.device(dev):
+        idx = torch.empty(n, ke, dtype=torch.int32, device=dev)
+        w = torch.empty(n, ke, dtype=torch.bfloat16, device=dev)
+        idx[:, :k], w[:, :k] = topk_idx, topk_w
+        r = Routes(torch.empty(n, ke, dtype=torch.int32, device=dev), w, torch.zeros(et, dtype=torch.int32, device=dev),
+                   torch.zeros(et + 1, dtype=torch.int32, device=dev), torch.empty(rows, dtype=torch.int32, device=dev),
+                   torch.zeros(4, dtype=torch.int32, device=dev), rows, n * ke)
+        if n and ke:
+            off = torch.empty(n, ke, dtype=torch.int32, device=dev)
+            row_w = torch.empty(rows, dtype=torch.bfloat16, device=dev)
+            scratch = torch.empty(_lib.lib().xmoe_route_pack_scratch_bytes(n, num_experts, num_shared), dtype=torch.uint8,
+                                  device=dev)
+            check(_lib.lib().xmoe_route_pack(idx.data_ptr(), w.data_ptr(), n, num_experts, k, ke, num_shared,
+                                             scratch.data_ptr(), r.counts.data_ptr(), r.offsets.data_ptr(), off.data_ptr(),
+                                             r.topk_row.data_ptr(), r.row_token.data_ptr(), row_w.data_ptr(),
+                                             r.status.data_ptr(), _stream()), "xmoe_route_pack")
+    return r
+
+
+def permute(x: torch.Tensor, topk_row: torch.Tensor, num_rows: int | None = None,
+            out: torch.Tensor | None = None) -> torch.Tensor:
+    """Tokens to rows sorted by expert: rows[topk_row[t, s]] = x[t]. x [N, H] bf16 / fp16 / fp32, contiguous; topk_row
+    int32 [N, k], an entry outside the rows is a slot without a row, no row is named twice. `out` [num_rows, H] keeps the
+    rows that no slot names; without it they are zero. Differentiable in x (without `out`)."""
+    if out is None:
+        if num_rows is None:
+            raise RuntimeError("permute needs num_rows or out")
+        if torch.is_grad_enabled() and x.requires_grad:
+            return _Permute.apply(x, topk_row, num_rows)
+        out = torch.zeros(num_rows, x.shape[-1], dtype=x.dtype, device=x.device)
+    elif torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
+        raise RuntimeError("permute into `out` is not differentiable: leave out away")
+    torch_ops.load()
+    torch.ops.xmoe_b200.permute(x, topk_row, out)
+    return out
+
+
+def permute_backward(drows: torch.Tensor, topk_row: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of permute's x: dx[t] = sum_s drows[topk_row[t, s]]."""
+    return unpermute(drows, topk_row, None, out)
+
+
+def unpermute(rows: torch.Tensor, topk_row: torch.Tensor, weights: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows back to tokens: y[t] = sum_s weights[t, s] * rows[topk_row[t, s]], fp32 in slot order, rounded once. weights
+    bf16 / fp32 [N, k] or None (1). `combine` is the bf16 form without weights that the fused layer ends with.
+    Differentiable in rows and weights (without `out`)."""
+    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+        if out is not None:
+            raise RuntimeError("unpermute into `out` is not differentiable: leave out away")
+        return _Unpermute.apply(rows, topk_row, weights)
+    if out is None:
+        out = torch.empty(topk_row.shape[0], rows.shape[-1], dtype=rows.dtype, device=rows.device)
+    torch_ops.load()
+    torch.ops.xmoe_b200.unpermute(rows, topk_row, weights, out)
+    return out
+
+
+def unpermute_backward(dy: torch.Tensor, rows: torch.Tensor, topk_row: torch.Tensor, weights: torch.Tensor | None = None,
+                       out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The gradients of unpermute: (drows, like rows; dweights fp32 [N, k]). drows[topk_row[t, s]] = weights[t, s] * dy[t],
+    dweights[t, s] = <dy[t], rows[topk_row[t, s]]>. `out` receives drows and keeps the rows that no slot names; without it
+    they are zero. No row may be named twice."""
+    drows = torch.zeros_like(rows) if out is None else out
+    dw = torch.empty(topk_row.shape, dtype=torch.float32, device=dy.device)
+    torch_ops.load()
+    torch.ops.xmoe_b200.unpermute_backward(dy, rows, topk_row, weights, drows, dw)
+    return drows, dw
+
+
+class _Permute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, topk_row, num_rows):
+        ctx.save_for_backward(topk_row)
+        with torch.no_grad():
+            return permute(x, topk_row, num_rows)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, drows):
+        return permute_backward(drows.contiguous(), *ctx.saved_tensors), None, None
+
+
+class _Unpermute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, topk_row, weights):
+        ctx.save_for_backward(rows, topk_row, weights)
+        with torch.no_grad():
+            return unpermute(rows, topk_row, weights)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        rows, topk_row, weights = ctx.saved_tensors
+        drows, dw = unpermute_backward(dy.contiguous(), rows, topk_row, weights)
+        return drows, None, None if weights is None else dw.to(weights.dtype)
 
 
 STAGE_NAMES = ("router", "route_pack", "act_amax", "act_quant", "ff1", "act_topk", "ff2", "combine")
