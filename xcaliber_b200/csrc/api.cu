@@ -665,7 +665,7 @@ int run_fp8_gemm(const void* x, int ldx, const float* x_scale, int lds, const vo
     int rc = make_tmap_codes(&a.tm_w, w, (uint64_t)k, (uint64_t)n, (uint64_t)mats, (uint64_t)ldw,
                              mats > 1 ? (uint64_t)w_mat_stride : (uint64_t)ldw * (uint64_t)n, 128);
     if (rc) return rc;
-    rc = make_tmap_codes(&a.tm_x, x, (uint64_t)contraction, (uint64_t)rows, 0, (uint64_t)ldx, 0, (uint32_t)tile);
+    rc = make_tmap_codes(&a.tm_x, x, (uint64_t)contraction, (uint64_t)rows, 0, (uint64_t)ldx, 0, (uint32_t)(tile == 256 ? 128 : tile));
     if (rc) return rc;
     a.x_scale = x_scale;
     a.w_scale = w_scale;
@@ -679,6 +679,7 @@ int run_fp8_gemm(const void* x, int ldx, const float* x_scale, int lds, const vo
     a.out_features = features;
     a.contraction = contraction;
     a.out_dtype = out_dtype;
+    a.out_vec = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)ldo * (out_dtype == XMOE_FP32 ? 4 : 2)) & 15u) == 0;
     a.num_sms = num_sms();
     return launch_fp8_gemm(a, tile, transpose, stream);
 }

@@ -14,8 +14,11 @@
 // tokens costs a narrow MMA instead of a mostly empty one. TRANS reads the same 128 x 128 weight box from shared memory
 // with the operand's transpose bit (features contiguous), so one copy of the weight serves both directions.
 //
-// Roles: warp 0 TMA producer, warp 1 tensor-memory owner and MMA issuer, warps 4.. epilogue (two per lane quadrant from
-// 128 tokens on). Every wait is bounded; a wait that gives up is reported by xmoe_fp8_status.
+// (up to 128 tokens per tile; larger ones run on CTA pairs with the roles exchanged, see below).
+//
+// Roles: warp 0 TMA producer, warp 1 tensor-memory owner and MMA issuer, warps 2-3 scales, warps 4.. epilogue (two per
+// lane quadrant for 128 tokens). Every wait is bounded; a wait that gives up is reported by xmoe_fp8_status.
+#include "cluster.cuh"
 #include "elem.cuh"
 #include "kernels.h"
 #include "tile_sched.cuh"
@@ -31,20 +34,29 @@ constexpr int kMaxMats = 1032;
 constexpr int kBoxBytes = 128 * 128;  // weight box of one block
 constexpr uint32_t kBadSegment = 0x700u;
 
+template <bool PAIR>
 __device__ __forceinline__ void mma_fp8(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "mov.b64 da, {%1, %5};\n\t"
-        "mov.b64 db, {%2, %5};\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw128)
-        : "memory");
+#define XMOE_MMA_FP8(GROUP)                                                                                            \
+    asm volatile(                                                                                                      \
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"                                                                    \
+        "mov.b64 da, {%1, %5};\n\t"                                                                                    \
+        "mov.b64 db, {%2, %5};\n\t"                                                                                    \
+        "setp.ne.b32 p, %4, 0;\n\t"                                                                                    \
+        "tcgen05.mma.cta_group::" GROUP ".kind::f8f6f4 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),                        \
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHiSw128)                                           \
+        : "memory")
+    if (PAIR) XMOE_MMA_FP8("2");
+    else XMOE_MMA_FP8("1");
+#undef XMOE_MMA_FP8
 }
-// kind::f8f6f4: accumulator fp32 [4,6) = 1, a/b format e4m3 = 0, transposed A [15], N>>3 [17,23), M>>4 [24,29)
-__host__ __device__ constexpr uint32_t idesc_fp8(uint32_t m, uint32_t n, bool a_trans) {
-    return (1u << 4) | ((a_trans ? 1u : 0u) << 15) | ((n >> 3) << 17) | ((m >> 4) << 24);
+// kind::f8f6f4: accumulator fp32 [4,6) = 1, a/b format e4m3 = 0, transposed A [15] / B [16], N>>3 [17,23), M>>4 [24,29)
+__host__ __device__ constexpr uint32_t idesc_fp8(uint32_t m, uint32_t n, bool a_trans, bool b_trans) {
+    return (1u << 4) | ((a_trans ? 1u : 0u) << 15) | ((b_trans ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
+// A transposed operand (features contiguous): a K step of 32 is 32 rows of 128 bytes; both stride fields are the 1024
+// bytes between 8-row groups (the tile is one swizzle atom wide, so only one of them is used).
+__device__ __forceinline__ uint32_t desc_lo_trans(uint32_t smem_addr) { return ((smem_addr & 0x3ffffu) >> 4) | ((1024u >> 4) << 16); }
+constexpr uint32_t kTransStep = (32u * 128u) >> 4;
 // a * b + c on two fp32 at once
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 d;
@@ -55,15 +67,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return d;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
-        "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
-        "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
 
 template <int TN>
 struct Cfg {
@@ -71,36 +74,72 @@ struct Cfg {
     static constexpr int kThreads = 128 + 32 * kEpiWarps;
     static constexpr int kCols = TN / (kEpiWarps / 4);            // token columns per epilogue warp
     static constexpr int kChunk = kCols < 32 ? 16 : 32;           // columns per tensor-memory read
-    static constexpr int kAcc = TN >= 256 ? 2 : 4;                // accumulators in tensor memory
-    static constexpr int kTmemCols = kAcc * TN < 64 ? 64 : kAcc * TN;
+    static constexpr int kAcc = 4;                                // accumulators in tensor memory
+    static constexpr int kTmemCols = kAcc * TN;
     static constexpr int kStageBytes = kBoxBytes + TN * 128;
-    static constexpr int kStages = TN >= 256 ? 4 : (TN >= 128 ? 6 : (TN >= 64 ? 8 : 10));
-    // a scale slot is written again kStages + kAcc blocks later: by then the MMA of the block that used the stage
-    // kStages blocks ago has been issued, so the epilogue has drained the block kAcc before that one
-    static constexpr int kScaleSlots = kStages + kAcc;
-    static constexpr size_t kTail = (size_t)kScaleSlots * TN * 4 + 1024;
+    static constexpr int kStages = TN >= 128 ? 6 : (TN >= 64 ? 8 : 10);
+    // scale slots run further ahead than the accumulators: at the start of a tile the first scales come from global memory
+    static constexpr int kSlots = TN >= 128 ? 8 : 16;
+    static constexpr size_t kTail = (size_t)kSlots * TN * 4 + 1024;
     static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kTail + (size_t)(3 * kMaxMats + 4) * 4;
     static_assert(kSmem <= 232448, "shared memory");
-    static_assert(kTmemCols <= 512, "tensor memory");
+    static_assert(kTmemCols >= 32 && kTmemCols <= 512, "tensor memory");
 };
+
+// The experts' segments, kept inside the buffers: a segment that does not start at a multiple of 16 rows inside them
+// counts as empty (and is reported), one that runs past the end is cut.
+__device__ __forceinline__ void load_segments(const Fp8GemmArgs& a, int* counts, int* offsets, int threads) {
+    for (int e = threadIdx.x; e < a.mats; e += threads) {
+        int c = a.counts ? a.counts[e] : a.rows, o = a.counts ? a.offsets[e] : 0;
+        if (c > 0 && (o < 0 || o >= a.rows || (o & 15))) {
+            atomicCAS(&g_fp8_status, 0u, kBadSegment);
+            c = 0;
+        }
+        counts[e] = c <= 0 ? 0 : min(c, a.rows - o);
+        offsets[e] = o;
+    }
+}
+
+// Completes the tensor-memory reads issued so far; naming the registers keeps their uses behind the wait.
+template <int N>
+__device__ __forceinline__ void tmem_wait_for(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+template <int N>
+__device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t* r) {
+    if (N == 32) tmem_ld32(taddr, r);
+    else tmem_ld16(taddr, r);
+}
+// sums += v * scale over N columns; the scales come from shared memory, the same for all lanes
+template <int N>
+__device__ __forceinline__ void add_scaled(float2* sum, const uint32_t* v, const float4* scale) {
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+        const float4 s = scale[j];
+        sum[2 * j] = fma2(make_float2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])), make_float2(s.x, s.y), sum[2 * j]);
+        sum[2 * j + 1] = fma2(make_float2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])), make_float2(s.z, s.w), sum[2 * j + 1]);
+    }
+}
 
 template <int TN, bool TRANS, typename OT>
 __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __grid_constant__ Fp8GemmArgs a) {
     using C = Cfg<TN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    float* scales = reinterpret_cast<float*>(smem + (size_t)C::kStages * C::kStageBytes);
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(scales + C::kScaleSlots * TN);
+    float* scales = reinterpret_cast<float*>(smem + (size_t)C::kStages * C::kStageBytes);  // [kSlots][TN] token scale * weight scale
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(scales + C::kSlots * TN);
     uint64_t* empty_bar = full_bar + 16;
-    uint64_t* sc_full = empty_bar + 16;  // [kScaleSlots]
-    uint64_t* acc_full = sc_full + 16;
+    uint64_t* sc_full = empty_bar + 16;  // [kSlots] a block's scales are written (2 warps)
+    uint64_t* sc_empty = sc_full + 16;   // [kSlots] ... and used by this CTA's epilogue warps
+    uint64_t* acc_full = sc_empty + 16;
     uint64_t* acc_empty = acc_full + 4;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 4);
     volatile uint32_t* abort_flag = tmem_slot + 1;
     int* counts = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full_bar) + 1024);
     int* offsets = counts + kMaxMats;
     int* prefix = offsets + kMaxMats;
-    static_assert(C::kScaleSlots <= 16, "barrier block");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int w_tiles = (a.out_features + 127) / 128;
@@ -111,7 +150,10 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
         }
-        for (int s = 0; s < C::kScaleSlots; ++s) mbar_init(&sc_full[s], 1);
+        for (int s = 0; s < C::kSlots; ++s) {
+            mbar_init(&sc_full[s], 2);
+            mbar_init(&sc_empty[s], C::kEpiWarps);
+        }
         for (int s = 0; s < C::kAcc; ++s) {
             mbar_init(&acc_full[s], 1);
             mbar_init(&acc_empty[s], C::kEpiWarps);
@@ -125,17 +167,7 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
         tmem_alloc(tmem_slot, C::kTmemCols);
         tmem_relinquish();
     }
-    // the experts' segments, kept inside the buffers: a segment that does not start at a multiple of 16 rows inside
-    // them counts as empty (and is reported), one that runs past the end is cut
-    for (int e = threadIdx.x; e < a.mats; e += C::kThreads) {
-        int c = a.counts ? a.counts[e] : a.rows, o = a.counts ? a.offsets[e] : 0;
-        if (c > 0 && (o < 0 || o >= a.rows || (o & 15))) {
-            atomicCAS(&g_fp8_status, 0u, kBadSegment);
-            c = 0;
-        }
-        counts[e] = c <= 0 ? 0 : min(c, a.rows - o);
-        offsets[e] = o;
-    }
+    load_segments(a, counts, offsets, C::kThreads);
     tc_fence_before();
     __syncthreads();
     if (warp == 2) tile_prefix_build(prefix, counts, a.mats, w_tiles, TN);
@@ -146,115 +178,146 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
     const int stride = balanced_stride(total_tiles, gridDim.x);
     const int first = (int)blockIdx.x < stride ? (int)blockIdx.x : total_tiles;
 
-    if (warp == 0) {
-        if (lane == 0) {
-            uint32_t s = 0, ph = 0, slot = 0;
-            bool ok = true;
-            for (int item = first; item < total_tiles && ok; item += stride) {
-                const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, TN);
-                // scales of this tile's tokens: a multiple of 16 bytes, inside the block's row (lds >= rows, both ends
-                // multiples of 4)
-                const uint32_t sc_bytes = (uint32_t)min(TN, ((a.rows + 3) & ~3) - t.row0) * 4u;
-                const float* sc = a.x_scale + t.row0;
-                for (int kb = 0; kb < kb_total; ++kb) {
-                    if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_MMA)) {
-                        ok = false;
-                        break;
+    if (warp < 4) {
+        if (warp == 0) {
+            if (lane == 0) {
+                uint32_t s = 0, ph = 0;
+                bool ok = true;
+                for (int item = first; item < total_tiles && ok; item += stride) {
+                    const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, TN);
+                    for (int kb = 0; kb < kb_total; ++kb) {
+                        if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_MMA)) {
+                            ok = false;
+                            break;
+                        }
+                        uint8_t* st = smem + (size_t)s * C::kStageBytes;
+                        mbar_expect_tx(&full_bar[s], C::kStageBytes);
+                        if (TRANS) tma_load_3d(st, &a.tm_w, t.wt * 128, kb * 128, t.e, &full_bar[s]);
+                        else tma_load_3d(st, &a.tm_w, kb * 128, t.wt * 128, t.e, &full_bar[s]);
+                        tma_load_2d(st + kBoxBytes, &a.tm_x, kb * 128, t.row0, &full_bar[s]);
+                        if (++s == (uint32_t)C::kStages) { s = 0; ph ^= 1u; }
                     }
-                    uint8_t* st = smem + (size_t)s * C::kStageBytes;
-                    mbar_expect_tx(&full_bar[s], C::kStageBytes);
-                    if (TRANS) tma_load_3d(st, &a.tm_w, t.wt * 128, kb * 128, t.e, &full_bar[s]);
-                    else tma_load_3d(st, &a.tm_w, kb * 128, t.wt * 128, t.e, &full_bar[s]);
-                    tma_load_2d(st + kBoxBytes, &a.tm_x, kb * 128, t.row0, &full_bar[s]);
-                    mbar_expect_tx(&sc_full[slot], sc_bytes);
-                    tma_load_1d(scales + slot * TN, sc + (size_t)kb * a.lds, sc_bytes, &sc_full[slot]);
-                    if (++s == (uint32_t)C::kStages) { s = 0; ph ^= 1u; }
-                    if (++slot == (uint32_t)C::kScaleSlots) slot = 0;
                 }
             }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t kStage16 = C::kStageBytes >> 4;
-            // K-major: 32 values further along K are 32 bytes inside the swizzle row. TRANS: features are contiguous,
-            // a K step of 32 is 32 rows of 128 bytes; both stride fields are the 1024 bytes between 8-row groups (the
-            // tile is one swizzle atom wide, so only one of them is used).
-            const uint32_t w_lo0 = TRANS ? ((smem_u32(smem) & 0x3ffffu) >> 4) | ((1024u >> 4) << 16) : umma_desc_lo_sw128(smem_u32(smem));
-            const uint32_t x_lo0 = umma_desc_lo_sw128(smem_u32(smem + kBoxBytes));
-            constexpr uint32_t kWStep = TRANS ? (32u * 128u) >> 4 : 2u;
-            uint32_t s = 0, ph = 0, acc = 0, acc_ph = 0;
-            bool ok = true;
-            for (int item = first; item < total_tiles && ok; item += stride) {
-                const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, TN);
-                const int n_mma = (min(TN, t.count - t.nt_idx * TN) + 15) & ~15;
-                const uint32_t idesc = idesc_fp8(128, (uint32_t)n_mma, TRANS);
-                for (int kb = 0; kb < kb_total; ++kb) {
-                    if (!mbar_wait(&acc_empty[acc], acc_ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_EPI) ||
-                        !mbar_wait(&full_bar[s], ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t w_lo = w_lo0 + s * kStage16, x_lo = x_lo0 + s * kStage16;
+        } else if (warp == 1) {
+            if (lane == 0) {
+                constexpr uint32_t kStage16 = C::kStageBytes >> 4;
+                const uint32_t w_lo0 = TRANS ? desc_lo_trans(smem_u32(smem)) : umma_desc_lo_sw128(smem_u32(smem));
+                const uint32_t x_lo0 = umma_desc_lo_sw128(smem_u32(smem + kBoxBytes));
+                constexpr uint32_t kWStep = TRANS ? kTransStep : 2u;  // K-major: 32 bytes inside the swizzle row
+                uint32_t s = 0, ph = 0, acc = 0, acc_ph = 0;
+                bool ok = true;
+                for (int item = first; item < total_tiles && ok; item += stride) {
+                    const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, TN);
+                    const int n_tok = min(TN, t.count - t.nt_idx * TN);
+                    const uint32_t idesc = idesc_fp8(128, (uint32_t)((n_tok + 15) & ~15), TRANS, false);
+                    for (int kb = 0; kb < kb_total; ++kb) {
+                        if (!mbar_wait(&acc_empty[acc], acc_ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_EPI) ||
+                            !mbar_wait(&full_bar[s], ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t w_lo = w_lo0 + s * kStage16, x_lo = x_lo0 + s * kStage16;
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        mma_fp8(tmem_base + acc * TN, w_lo + kk * kWStep, x_lo + kk * 2, idesc, kk ? 1u : 0u);
-                    tc_commit(&empty_bar[s]);
-                    tc_commit(&acc_full[acc]);
-                    if (++s == (uint32_t)C::kStages) { s = 0; ph ^= 1u; }
-                    if (++acc == (uint32_t)C::kAcc) { acc = 0; acc_ph ^= 1u; }
+                        for (int kk = 0; kk < 4; ++kk)
+                            mma_fp8<false>(tmem_base + acc * TN, w_lo + kk * kWStep, x_lo + kk * 2, idesc, kk ? 1u : 0u);
+                        tc_commit(&empty_bar[s]);
+                        tc_commit(&acc_full[acc]);
+                        if (++s == (uint32_t)C::kStages) { s = 0; ph ^= 1u; }
+                        if (++acc == (uint32_t)C::kAcc) { acc = 0; acc_ph ^= 1u; }
+                    }
+                }
+            }
+        } else {
+            // Scales: per block, token scale * weight scale into a ring in shared memory. Each thread
+            // keeps the token scales of the next blocks in flight in registers (global loads, mostly from L2).
+            constexpr int kPer = (TN + 63) / 64, kAhead = 4;
+            const int t64 = threadIdx.x - 64;
+            uint32_t slot = 0, slot_ph = 0;
+            bool ok = true;
+            for (int item = first; item < total_tiles && ok; item += stride) {
+                const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, TN);
+                const int n_tok = min(TN, t.count - t.nt_idx * TN);
+                const float* ws = a.w_scale + (size_t)t.e * w_tiles * kb_total + (TRANS ? (size_t)t.wt : (size_t)t.wt * kb_total);
+                const size_t ws_step = TRANS ? w_tiles : 1;
+                const float* xs = a.x_scale + t.row0 + t64;
+                float x[kAhead][kPer], w[kAhead];
+                auto fetch = [&](int kb, int i) {
+                    if (kb >= kb_total) return;
+                    w[i] = ws[kb * ws_step];
+#pragma unroll
+                    for (int p = 0; p < kPer; ++p) x[i][p] = t64 + p * 64 < n_tok ? xs[(size_t)kb * a.lds + p * 64] : 0.f;
+                };
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) fetch(i, i);
+                for (int kb0 = 0; kb0 < kb_total && ok; kb0 += kAhead) {
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i) {
+                        if (kb0 + i < kb_total && ok) {
+                            ok = mbar_wait(&sc_empty[slot], slot_ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_EPI);
+#pragma unroll
+                            for (int p = 0; p < kPer; ++p)
+                                if (t64 + p * 64 < TN) scales[slot * TN + t64 + p * 64] = x[i][p] * w[i];
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&sc_full[slot]);
+                            fetch(kb0 + i + kAhead, i);
+                            if (++slot == (uint32_t)C::kSlots) { slot = 0; slot_ph ^= 1u; }
+                        }
+                    }
                 }
             }
         }
-    } else if (warp >= 4) {
+    } else {
         const int q = warp & 3, part = (warp - 4) >> 2;
         const int col0 = part * C::kCols;
         const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16) + col0;
-        const int ws_ld = TRANS ? w_tiles : kb_total;  // row length of a matrix's scale table
         uint32_t acc = 0, acc_ph = 0, slot = 0, slot_ph = 0;
         bool ok = true;
         for (int item = first; item < total_tiles && ok; item += stride) {
             const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, TN);
             const int n_tok = min(TN, t.count - t.nt_idx * TN) - col0;  // this warp's live columns (may be <= 0)
-            const float* ws = a.w_scale + (size_t)t.e * w_tiles * kb_total + (TRANS ? t.wt : t.wt * ws_ld);
             float2 sum[C::kCols / 2];
 #pragma unroll
             for (int j = 0; j < C::kCols / 2; ++j) sum[j] = make_float2(0.f, 0.f);
-            float ws_lane = 0.f;
             for (int kb = 0; kb < kb_total; ++kb) {
-                if ((kb & 31) == 0) ws_lane = kb + lane < kb_total ? ws[(size_t)(kb + lane) * (TRANS ? ws_ld : 1)] : 0.f;
-                const float sw = __shfl_sync(0xffffffffu, ws_lane, kb & 31);
-                if (!mbar_wait(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA) ||
+                if (!mbar_wait(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_DQ) ||
                     !mbar_wait(&acc_full[acc], acc_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_ACC)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
                 const float4* xs = reinterpret_cast<const float4*>(scales + slot * TN + col0);
+                const uint32_t src = lane_addr + acc * TN;
+                constexpr int kN = C::kCols / C::kChunk;
+                if (n_tok > C::kCols - C::kChunk) {  // all chunks hold tokens: the next read is in flight while one is added
+                    uint32_t v[2][C::kChunk];
+                    tmem_read<C::kChunk>(src, v[0]);
 #pragma unroll
-                for (int c = 0; c < C::kCols / C::kChunk; ++c) {
-                    if (c * C::kChunk < n_tok) {
-                        uint32_t v[C::kChunk];
-                        if (C::kChunk == 32) tmem_ld32(lane_addr + acc * TN + c * C::kChunk, v);
-                        else tmem_ld16(lane_addr + acc * TN + c * C::kChunk, v);
-                        tmem_ld_wait();
+                    for (int c = 0; c < kN; ++c) {
+                        tmem_wait_for<C::kChunk>(v[c & 1]);
+                        if (c + 1 < kN) tmem_read<C::kChunk>(src + (c + 1) * C::kChunk, v[(c + 1) & 1]);
+                        add_scaled<C::kChunk>(sum + c * C::kChunk / 2, v[c & 1], xs + c * C::kChunk / 4);
+                    }
+                } else {
 #pragma unroll
-                        for (int j = 0; j < C::kChunk / 4; ++j) {
-                            const float4 x4 = xs[c * (C::kChunk / 4) + j];
-                            float2* d = &sum[(c * C::kChunk + 4 * j) / 2];
-                            const float2 sw2 = make_float2(sw, sw);
-                            d[0] = fma2(make_float2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])),
-                                        mul2(make_float2(x4.x, x4.y), sw2), d[0]);
-                            d[1] = fma2(make_float2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])),
-                                        mul2(make_float2(x4.z, x4.w), sw2), d[1]);
+                    for (int c = 0; c < kN; ++c) {
+                        if (c * C::kChunk < n_tok) {
+                            uint32_t v[C::kChunk];
+                            tmem_read<C::kChunk>(src + c * C::kChunk, v);
+                            tmem_wait_for<C::kChunk>(v);
+                            add_scaled<C::kChunk>(sum + c * C::kChunk / 2, v, xs + c * C::kChunk / 4);
                         }
                     }
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_empty[acc]);
+                if (lane == 0) {
+                    mbar_arrive(&sc_empty[slot]);
+                    mbar_arrive(&acc_empty[acc]);
+                }
                 if (++acc == (uint32_t)C::kAcc) { acc = 0; acc_ph ^= 1u; }
-                if (++slot == (uint32_t)C::kScaleSlots) { slot = 0; slot_ph ^= 1u; }
+                if (++slot == (uint32_t)C::kSlots) { slot = 0; slot_ph ^= 1u; }
             }
             if (!ok) break;
             const int f = t.wt * 128 + q * 32 + lane;
@@ -276,36 +339,293 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
     if (warp == 1) tmem_dealloc(tmem_base, C::kTmemCols);
 }
 
+// ---- 256 tokens x 256 features on CTA pairs --------------------------------------------------------------------------
+// From 128 tokens per expert on the product is bound by arithmetic, and what decides is the epilogue: per block and SM
+// 128 x 256 values are read from tensor memory, scaled and added. Here tokens are the MMA's M side (a lane = a token) and
+// the features its N side, so a thread's token scale is one register and the weight's scale one number per warp (an
+// epilogue warp owns 128 features, one scale block): one multiplication per thread and block, then one packed FMA per two
+// values. With the tokens on the N side every value needs its own scale from shared memory, which the MMA's operand reads
+// keep busy: 4096 x 4096 x 7168 took 210 us that way, 159 with the scale reads left out.
+// Each CTA of the pair stages its 128 tokens and 128 of the 256 features: 32 KB per 128 columns of K instead of 48.
+constexpr int kPairStages = 6, kPairThreads = 384, kPairEpiWarps = 8;
+constexpr int kPairStageBytes = 2 * kBoxBytes;
+constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStageBytes + 1024 + (size_t)(3 * kMaxMats + 4) * 4;
+static_assert(kPairSmem <= 232448, "shared memory");
+// 128 sums and two 32-column reads per epilogue thread: these warps take registers over from the single-purpose ones. 384
+// threads are launched with 168 each; 128 * 40 + 256 * 232 = 384 * 168.
+constexpr int kRegsFew = 40, kRegsEpi = 232;
+static_assert(128 * kRegsFew + 256 * kRegsEpi <= 384 * 168, "register pool");
+
+__device__ __forceinline__ void add_scaled32(float2* sum, const uint32_t* v, float2 scale) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        sum[j] = fma2(make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1])), scale, sum[j]);
+}
+
+template <bool TRANS, typename OT>
+__global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __grid_constant__ Fp8GemmArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + (size_t)kPairStages * kPairStageBytes);
+    uint64_t* empty_bar = full_bar + 8;
+    uint64_t* acc_full = empty_bar + 8;  // [2] in each CTA
+    uint64_t* acc_empty = acc_full + 2;  // [2] leader: both CTAs' epilogue warps
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile uint32_t* abort_flag = tmem_slot + 1;
+    int* counts = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full_bar) + 1024);
+    int* offsets = counts + kMaxMats;
+    int* prefix = offsets + kMaxMats;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_ctarank();
+    const int w_blocks = (a.out_features + 127) / 128, w_tiles = (w_blocks + 1) / 2;
+    const int kb_total = (a.contraction + 127) / 128;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPairStages; ++s) {
+            mbar_init(&full_bar[s], rank == 0 ? 2 : 1);  // leader: + the peer's report that its stage landed
+            mbar_init(&empty_bar[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&acc_full[s], 1);
+            mbar_init(&acc_empty[s], 2 * kPairEpiWarps);
+        }
+        *abort_flag = 0u;
+        mbar_fence_init();
+        prefetch_tmap(&a.tm_w);
+        prefetch_tmap(&a.tm_x);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
+    }
+    load_segments(a, counts, offsets, kPairThreads);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) tile_prefix_build(prefix, counts, a.mats, w_tiles, 256);
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int total_tiles = prefix[a.mats];
+    const int stride = balanced_stride(total_tiles, (int)gridDim.x >> 1);
+    const int first = ((int)blockIdx.x >> 1) < stride ? (int)blockIdx.x >> 1 : total_tiles;
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
+        if (warp == 0 && lane == 0) {
+            uint32_t s = 0, ph = 0;
+            bool ok = true;
+            for (int item = first; item < total_tiles && ok; item += stride) {
+                const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, 256);
+                const int f0 = t.wt * 256 + rank * 128, row = t.row0 + rank * 128;
+                for (int kb = 0; kb < kb_total; ++kb) {
+                    if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_MMA)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* st = smem + (size_t)s * kPairStageBytes;
+                    mbar_expect_tx(&full_bar[s], kPairStageBytes);
+                    tma_load_2d(st, &a.tm_x, kb * 128, row, &full_bar[s]);
+                    if (TRANS) tma_load_3d(st + kBoxBytes, &a.tm_w, f0, kb * 128, t.e, &full_bar[s]);
+                    else tma_load_3d(st + kBoxBytes, &a.tm_w, kb * 128, f0, t.e, &full_bar[s]);
+                    if (++s == (uint32_t)kPairStages) { s = 0; ph ^= 1u; }
+                }
+            }
+        } else if (warp == 1 && lane == 0 && rank == 0) {
+            constexpr uint32_t kStage16 = kPairStageBytes >> 4;
+            constexpr uint32_t idesc = idesc_fp8(256, 256, false, TRANS);
+            constexpr uint32_t kWStep = TRANS ? kTransStep : 2u;
+            const uint32_t x_lo0 = umma_desc_lo_sw128(smem_u32(smem));
+            const uint32_t w_lo0 = TRANS ? desc_lo_trans(smem_u32(smem + kBoxBytes)) : umma_desc_lo_sw128(smem_u32(smem + kBoxBytes));
+            uint32_t s = 0, ph = 0, acc = 0, acc_ph = 0;
+            bool ok = true;
+            for (int item = first; item < total_tiles && ok; item += stride) {
+                for (int kb = 0; kb < kb_total; ++kb) {
+                    if (!mbar_wait(&acc_empty[acc], acc_ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_EPI) ||
+                        !mbar_wait(&full_bar[s], ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t w_lo = w_lo0 + s * kStage16, x_lo = x_lo0 + s * kStage16;
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        mma_fp8<true>(tmem_base + acc * 256, x_lo + kk * 2, w_lo + kk * kWStep, idesc, kk ? 1u : 0u);
+                    tc_commit_pair_mask(smem_u32(&empty_bar[s]), 3);
+                    tc_commit_pair_mask(smem_u32(&acc_full[acc]), 3);
+                    if (++s == (uint32_t)kPairStages) { s = 0; ph ^= 1u; }
+                    acc ^= 1u;
+                    acc_ph ^= acc ^ 1u;
+                }
+            }
+        } else if (warp == 1 && lane == 0) {
+            // the peer reports its landed stages to the leader
+            uint32_t s = 0, ph = 0;
+            bool ok = true;
+            for (int item = first; item < total_tiles && ok; item += stride) {
+                for (int kb = 0; kb < kb_total; ++kb) {
+                    if (!mbar_wait(&full_bar[s], ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
+                        ok = false;
+                        break;
+                    }
+                    mbar_arrive_cluster(map_to_cta(smem_u32(&full_bar[s]), 0));
+                    if (++s == (uint32_t)kPairStages) { s = 0; ph ^= 1u; }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+        const int q = warp & 3, part = (warp - 4) >> 2;
+        const uint32_t src0 = tmem_base + ((uint32_t)(q * 32) << 16) + part * 128;
+        const uint32_t leader_empty = map_to_cta(smem_u32(acc_empty), 0);
+        uint32_t acc = 0, acc_ph = 0;
+        bool ok = true;
+        for (int item = first; item < total_tiles && ok; item += stride) {
+            const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, 256);
+            const int m = rank * 128 + q * 32 + lane;  // token of the tile
+            const bool live = m < t.count - t.nt_idx * 256;
+            const int fb = min(t.wt * 2 + part, w_blocks - 1);  // a block past the end: its values are not stored
+            const float* ws = a.w_scale + (size_t)t.e * w_blocks * kb_total + (TRANS ? (size_t)fb : (size_t)fb * kb_total);
+            const size_t ws_step = TRANS ? w_blocks : 1;
+            const float* xs = a.x_scale + (live ? t.row0 + m : 0);
+            // scales of the next two blocks are in flight
+            float x_next[2], w_next[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int kb = min(i, kb_total - 1);
+                x_next[i] = xs[(size_t)kb * a.lds];
+                w_next[i] = ws[kb * ws_step];
+            }
+            float2 sum[64];
+#pragma unroll
+            for (int j = 0; j < 64; ++j) sum[j] = make_float2(0.f, 0.f);
+            bool ready = false;
+            for (int kb0 = 0; kb0 < kb_total && ok; kb0 += 2) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (kb0 + i >= kb_total) break;
+                    if (!ready && !mbar_wait(&acc_full[acc], acc_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_ACC)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t src = src0 + acc * 256;
+                    uint32_t v0[32], v1[32];
+                    tmem_ld32(src, v0);
+                    const float s = x_next[i] * w_next[i];
+                    const float2 s2 = make_float2(s, s);
+                    {
+                        const int kb = min(kb0 + i + 2, kb_total - 1);
+                        x_next[i] = xs[(size_t)kb * a.lds];
+                        w_next[i] = ws[kb * ws_step];
+                    }
+                    tmem_wait_for<32>(v0);
+                    tmem_ld32(src + 32, v1);
+                    add_scaled32(sum, v0, s2);
+                    tmem_wait_for<32>(v1);
+                    tmem_ld32(src + 64, v0);
+                    add_scaled32(sum + 16, v1, s2);
+                    tmem_wait_for<32>(v0);
+                    tmem_ld32(src + 96, v1);
+                    add_scaled32(sum + 32, v0, s2);
+                    tmem_wait_for<32>(v1);
+                    // everything is in registers: hand the accumulator back, and look whether the next one is there
+                    // while the last columns are added
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(leader_empty + acc * 8u);
+                    acc ^= 1u;
+                    acc_ph ^= acc ^ 1u;
+                    ready = mbar_test_wait(&acc_full[acc], acc_ph);
+                    add_scaled32(sum + 48, v1, s2);
+                }
+            }
+            if (!ok) break;
+            const int f = t.wt * 256 + part * 128;
+            if (live && f < a.out_features) {
+                OT* dst = reinterpret_cast<OT*>(a.out) + (size_t)(t.row0 + m) * a.ldo + f;
+                constexpr int kVec = 16 / sizeof(OT);
+                if (a.out_vec && f + 128 <= a.out_features) {
+#pragma unroll
+                    for (int j = 0; j < 128; j += kVec) {
+                        Pack<OT, kVec> o;
+#pragma unroll
+                        for (int i = 0; i < kVec; ++i) o.v[i] = from_f32<OT>((j + i) & 1 ? sum[(j + i) / 2].y : sum[(j + i) / 2].x);
+                        store_pack<OT, kVec>(dst + j, o);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 128; ++j)
+                        if (f + j < a.out_features) dst[j] = from_f32<OT>(j & 1 ? sum[j / 2].y : sum[j / 2].x);
+                }
+            }
+        }
+    }
+
+    __syncthreads();
+    if (*abort_flag) {  // let copies in flight land before the shared memory is given back
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // the peer's barriers and tensor memory are in use until both are here
+    if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+}
+
+// Shared memory beyond the default limit has to be asked for once per kernel and device.
+template <typename K>
+bool allow_smem(K kernel, size_t bytes, bool* done) {
+    const int dev = device_slot();
+    if (dev < 0) return false;
+    if (!done[dev]) done[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess;
+    return done[dev];
+}
+// No more tiles than this can exist (the experts' rows are on the device).
+size_t most_tiles(const Fp8GemmArgs& a, int tokens, int features) {
+    const size_t row_tiles = (size_t)(a.rows + tokens - 1) / tokens + (a.counts ? a.mats : 0);
+    return row_tiles * (size_t)((a.out_features + features - 1) / features);
+}
+
+template <bool TRANS, typename OT>
+int launch_pair(const Fp8GemmArgs& a, cudaStream_t stream) {
+    static bool smem_ok[kMaxDevices] = {};
+    if (!allow_smem(fp8_gemm_pair_kernel<TRANS, OT>, kPairSmem, smem_ok)) return XMOE_ERR_CUDA;
+    const size_t tiles = most_tiles(a, 256, 256), pairs = a.num_sms / 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles < pairs ? tiles : pairs) * 2);
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = kPairSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel<TRANS, OT>, a) == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
+}
 template <int TN, bool TRANS, typename OT>
 int launch_t(const Fp8GemmArgs& a, cudaStream_t stream) {
-    static bool attr_set_dev[kMaxDevices] = {};
-    const int dev = device_slot();
-    if (dev < 0) return XMOE_ERR_CUDA;
-    if (!attr_set_dev[dev]) {
-        if (cudaFuncSetAttribute(fp8_gemm_kernel<TN, TRANS, OT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)Cfg<TN>::kSmem) != cudaSuccess)
-            return XMOE_ERR_CUDA;
-        attr_set_dev[dev] = true;
-    }
-    // no more CTAs than there can be tiles
-    const size_t row_tiles = (size_t)(a.rows + TN - 1) / TN + (a.counts ? a.mats : 0);
-    const size_t tiles = row_tiles * (size_t)((a.out_features + 127) / 128);
-    const int grid = tiles < (size_t)a.num_sms ? (int)tiles : a.num_sms;
-    fp8_gemm_kernel<TN, TRANS, OT><<<grid, Cfg<TN>::kThreads, Cfg<TN>::kSmem, stream>>>(a);
-    return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
-}
-template <int TN, bool TRANS>
-int launch_out(const Fp8GemmArgs& a, cudaStream_t stream) {
-    switch (a.out_dtype) {
-        case XMOE_BF16: return launch_t<TN, TRANS, __nv_bfloat16>(a, stream);
-        case XMOE_FP16: return launch_t<TN, TRANS, __half>(a, stream);
-        case XMOE_FP32: return launch_t<TN, TRANS, float>(a, stream);
-        default: return XMOE_ERR_SHAPE;
+    if constexpr (TN == 256) {
+        return launch_pair<TRANS, OT>(a, stream);
+    } else {
+        static bool smem_ok[kMaxDevices] = {};
+        if (!allow_smem(fp8_gemm_kernel<TN, TRANS, OT>, Cfg<TN>::kSmem, smem_ok)) return XMOE_ERR_CUDA;
+        const size_t tiles = most_tiles(a, TN, 128);
+        const int grid = tiles < (size_t)a.num_sms ? (int)tiles : a.num_sms;
+        fp8_gemm_kernel<TN, TRANS, OT><<<grid, Cfg<TN>::kThreads, Cfg<TN>::kSmem, stream>>>(a);
+        return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
     }
 }
 template <int TN>
-int launch_dir(const Fp8GemmArgs& a, bool transpose, cudaStream_t stream) {
-    return transpose ? launch_out<TN, true>(a, stream) : launch_out<TN, false>(a, stream);
+int launch_tile(const Fp8GemmArgs& a, bool transpose, cudaStream_t stream) {
+    switch (a.out_dtype) {
+        case XMOE_BF16: return transpose ? launch_t<TN, true, __nv_bfloat16>(a, stream) : launch_t<TN, false, __nv_bfloat16>(a, stream);
+        case XMOE_FP16: return transpose ? launch_t<TN, true, __half>(a, stream) : launch_t<TN, false, __half>(a, stream);
+        case XMOE_FP32: return transpose ? launch_t<TN, true, float>(a, stream) : launch_t<TN, false, float>(a, stream);
+        default: return XMOE_ERR_SHAPE;
+    }
 }
 
 }  // namespace
@@ -313,11 +633,11 @@ int launch_dir(const Fp8GemmArgs& a, bool transpose, cudaStream_t stream) {
 int launch_fp8_gemm(const Fp8GemmArgs& a, int token_tile, bool transpose, cudaStream_t stream) {
     if (a.mats > kMaxMats) return XMOE_ERR_LIMIT;
     switch (token_tile) {
-        case 16: return launch_dir<16>(a, transpose, stream);
-        case 32: return launch_dir<32>(a, transpose, stream);
-        case 64: return launch_dir<64>(a, transpose, stream);
-        case 128: return launch_dir<128>(a, transpose, stream);
-        case 256: return launch_dir<256>(a, transpose, stream);
+        case 16: return launch_tile<16>(a, transpose, stream);
+        case 32: return launch_tile<32>(a, transpose, stream);
+        case 64: return launch_tile<64>(a, transpose, stream);
+        case 128: return launch_tile<128>(a, transpose, stream);
+        case 256: return launch_tile<256>(a, transpose, stream);
         default: return XMOE_ERR_SHAPE;
     }
 }
