@@ -16,7 +16,7 @@
 //
 // (up to 128 tokens per tile; larger ones run on CTA pairs with the roles exchanged, see below).
 //
-// Roles: warp 0 TMA producer, warp 1 tensor-memory owner and MMA issuer, warps 2-3 scales, warps 4.. epilogue (two per
+// Roles: warp 0 TMA producer, warp 1 tensor-memory owner and MMA issuer, warp 2 the tile list, warps 4.. epilogue (two per
 // lane quadrant for 128 tokens). Every wait is bounded; a wait that gives up is reported by xmoe_fp8_status.
 #include "cluster.cuh"
 #include "elem.cuh"
@@ -68,6 +68,10 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     return d;
 }
 
+__device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+
 template <int TN>
 struct Cfg {
     static constexpr int kEpiWarps = TN >= 128 ? 8 : 4;
@@ -78,8 +82,9 @@ struct Cfg {
     static constexpr int kTmemCols = kAcc * TN;
     static constexpr int kStageBytes = kBoxBytes + TN * 128;
     static constexpr int kStages = TN >= 128 ? 6 : (TN >= 64 ? 8 : 10);
-    // scale slots run further ahead than the accumulators: at the start of a tile the first scales come from global memory
-    static constexpr int kSlots = TN >= 128 ? 8 : 16;
+    // a scale slot is written again kStages + kAcc blocks later: by then the MMA of the block that used the stage kStages
+    // blocks ago has been issued, so the epilogue has drained the block kAcc before that one
+    static constexpr int kSlots = kStages + kAcc;
     static constexpr size_t kTail = (size_t)kSlots * TN * 4 + 1024;
     static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kTail + (size_t)(3 * kMaxMats + 4) * 4;
     static_assert(kSmem <= 232448, "shared memory");
@@ -112,12 +117,12 @@ __device__ __forceinline__ void tmem_read(uint32_t taddr, uint32_t* r) {
     if (N == 32) tmem_ld32(taddr, r);
     else tmem_ld16(taddr, r);
 }
-// sums += v * scale over N columns; the scales come from shared memory, the same for all lanes
+// sums += v * (token scale * weight scale) over N columns; the token scales come from shared memory, the same for all lanes
 template <int N>
-__device__ __forceinline__ void add_scaled(float2* sum, const uint32_t* v, const float4* scale) {
+__device__ __forceinline__ void add_scaled(float2* sum, const uint32_t* v, const float4* scale, float sw) {
 #pragma unroll
     for (int j = 0; j < N / 4; ++j) {
-        const float4 s = scale[j];
+        const float4 x = scale[j], s = make_float4(x.x * sw, x.y * sw, x.z * sw, x.w * sw);
         sum[2 * j] = fma2(make_float2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])), make_float2(s.x, s.y), sum[2 * j]);
         sum[2 * j + 1] = fma2(make_float2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])), make_float2(s.z, s.w), sum[2 * j + 1]);
     }
@@ -128,12 +133,11 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
     using C = Cfg<TN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    float* scales = reinterpret_cast<float*>(smem + (size_t)C::kStages * C::kStageBytes);  // [kSlots][TN] token scale * weight scale
+    float* scales = reinterpret_cast<float*>(smem + (size_t)C::kStages * C::kStageBytes);  // [kSlots][TN] the block's token scales
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(scales + C::kSlots * TN);
     uint64_t* empty_bar = full_bar + 16;
-    uint64_t* sc_full = empty_bar + 16;  // [kSlots] a block's scales are written (2 warps)
-    uint64_t* sc_empty = sc_full + 16;   // [kSlots] ... and used by this CTA's epilogue warps
-    uint64_t* acc_full = sc_empty + 16;
+    uint64_t* sc_full = empty_bar + 16;  // [kSlots]
+    uint64_t* acc_full = sc_full + 16;
     uint64_t* acc_empty = acc_full + 4;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 4);
     volatile uint32_t* abort_flag = tmem_slot + 1;
@@ -150,10 +154,7 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
         }
-        for (int s = 0; s < C::kSlots; ++s) {
-            mbar_init(&sc_full[s], 2);
-            mbar_init(&sc_empty[s], C::kEpiWarps);
-        }
+        for (int s = 0; s < C::kSlots; ++s) mbar_init(&sc_full[s], 1);
         for (int s = 0; s < C::kAcc; ++s) {
             mbar_init(&acc_full[s], 1);
             mbar_init(&acc_empty[s], C::kEpiWarps);
@@ -175,17 +176,25 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = prefix[a.mats];
-    const int stride = balanced_stride(total_tiles, gridDim.x);
-    const int first = (int)blockIdx.x < stride ? (int)blockIdx.x : total_tiles;
+    // a.split > 1: the CTAs of a cluster share one tile, each takes a part of the contraction (a cluster per tile at most)
+    const int split = a.split, rank = split > 1 ? (int)cluster_ctarank() : 0;
+    const int kb_lo = kb_total * rank / split, kb_hi = kb_total * (rank + 1) / split;
+    const int units = (int)gridDim.x / split, unit = (int)blockIdx.x / split;
+    const int stride = split > 1 ? units : balanced_stride(total_tiles, units);
+    const int first = unit < stride ? unit : total_tiles;
 
     if (warp < 4) {
         if (warp == 0) {
             if (lane == 0) {
-                uint32_t s = 0, ph = 0;
+                uint32_t s = 0, ph = 0, slot = 0;
                 bool ok = true;
                 for (int item = first; item < total_tiles && ok; item += stride) {
                     const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, TN);
-                    for (int kb = 0; kb < kb_total; ++kb) {
+                    // scales of this tile's tokens: a multiple of 16 bytes, inside the block's row (lds >= rows, both ends
+                    // multiples of 4)
+                    const uint32_t sc_bytes = (uint32_t)min(TN, ((a.rows + 3) & ~3) - t.row0) * 4u;
+                    const float* sc = a.x_scale + t.row0;
+                    for (int kb = kb_lo; kb < kb_hi; ++kb) {
                         if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_MMA)) {
                             ok = false;
                             break;
@@ -195,7 +204,10 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
                         if (TRANS) tma_load_3d(st, &a.tm_w, t.wt * 128, kb * 128, t.e, &full_bar[s]);
                         else tma_load_3d(st, &a.tm_w, kb * 128, t.wt * 128, t.e, &full_bar[s]);
                         tma_load_2d(st + kBoxBytes, &a.tm_x, kb * 128, t.row0, &full_bar[s]);
+                        mbar_expect_tx(&sc_full[slot], sc_bytes);
+                        tma_load_1d(scales + slot * TN, sc + (size_t)kb * a.lds, sc_bytes, &sc_full[slot]);
                         if (++s == (uint32_t)C::kStages) { s = 0; ph ^= 1u; }
+                        if (++slot == (uint32_t)C::kSlots) slot = 0;
                     }
                 }
             }
@@ -211,7 +223,7 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
                     const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, TN);
                     const int n_tok = min(TN, t.count - t.nt_idx * TN);
                     const uint32_t idesc = idesc_fp8(128, (uint32_t)((n_tok + 15) & ~15), TRANS, false);
-                    for (int kb = 0; kb < kb_total; ++kb) {
+                    for (int kb = kb_lo; kb < kb_hi; ++kb) {
                         if (!mbar_wait(&acc_empty[acc], acc_ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_EPI) ||
                             !mbar_wait(&full_bar[s], ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
                             ok = false;
@@ -229,44 +241,11 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
                     }
                 }
             }
-        } else {
-            // Scales: per block, token scale * weight scale into a ring in shared memory. Each thread
-            // keeps the token scales of the next blocks in flight in registers (global loads, mostly from L2).
-            constexpr int kPer = (TN + 63) / 64, kAhead = 4;
-            const int t64 = threadIdx.x - 64;
-            uint32_t slot = 0, slot_ph = 0;
-            bool ok = true;
-            for (int item = first; item < total_tiles && ok; item += stride) {
-                const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, TN);
-                const int n_tok = min(TN, t.count - t.nt_idx * TN);
-                const float* ws = a.w_scale + (size_t)t.e * w_tiles * kb_total + (TRANS ? (size_t)t.wt : (size_t)t.wt * kb_total);
-                const size_t ws_step = TRANS ? w_tiles : 1;
-                const float* xs = a.x_scale + t.row0 + t64;
-                float x[kAhead][kPer], w[kAhead];
-                auto fetch = [&](int kb, int i) {
-                    if (kb >= kb_total) return;
-                    w[i] = ws[kb * ws_step];
-#pragma unroll
-                    for (int p = 0; p < kPer; ++p) x[i][p] = t64 + p * 64 < n_tok ? xs[(size_t)kb * a.lds + p * 64] : 0.f;
-                };
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) fetch(i, i);
-                for (int kb0 = 0; kb0 < kb_total && ok; kb0 += kAhead) {
-#pragma unroll
-                    for (int i = 0; i < kAhead; ++i) {
-                        if (kb0 + i < kb_total && ok) {
-                            ok = mbar_wait(&sc_empty[slot], slot_ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_EPI);
-#pragma unroll
-                            for (int p = 0; p < kPer; ++p)
-                                if (t64 + p * 64 < TN) scales[slot * TN + t64 + p * 64] = x[i][p] * w[i];
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&sc_full[slot]);
-                            fetch(kb0 + i + kAhead, i);
-                            if (++slot == (uint32_t)C::kSlots) { slot = 0; slot_ph ^= 1u; }
-                        }
-                    }
-                }
-            }
+        }
+        if (split > 1 && first < total_tiles) {  // the two barriers of the exchange below
+            __syncwarp();
+            cluster_sync_all();
+            cluster_sync_all();
         }
     } else {
         const int q = warp & 3, part = (warp - 4) >> 2;
@@ -277,11 +256,15 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
         for (int item = first; item < total_tiles && ok; item += stride) {
             const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, TN);
             const int n_tok = min(TN, t.count - t.nt_idx * TN) - col0;  // this warp's live columns (may be <= 0)
+            const float* ws = a.w_scale + (size_t)t.e * w_tiles * kb_total + (TRANS ? (size_t)t.wt : (size_t)t.wt * kb_total);
             float2 sum[C::kCols / 2];
 #pragma unroll
             for (int j = 0; j < C::kCols / 2; ++j) sum[j] = make_float2(0.f, 0.f);
-            for (int kb = 0; kb < kb_total; ++kb) {
-                if (!mbar_wait(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_DQ) ||
+            float ws_lane = 0.f;  // the weight's scales of 32 blocks, one per lane
+            for (int kb = kb_lo; kb < kb_hi; ++kb) {
+                if (((kb - kb_lo) & 31) == 0) ws_lane = kb + lane < kb_hi ? ws[(size_t)(kb + lane) * (TRANS ? w_tiles : 1)] : 0.f;
+                const float sw = __shfl_sync(0xffffffffu, ws_lane, (kb - kb_lo) & 31);
+                if (!mbar_wait(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA) ||
                     !mbar_wait(&acc_full[acc], acc_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_ACC)) {
                     ok = false;
                     break;
@@ -297,7 +280,7 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
                     for (int c = 0; c < kN; ++c) {
                         tmem_wait_for<C::kChunk>(v[c & 1]);
                         if (c + 1 < kN) tmem_read<C::kChunk>(src + (c + 1) * C::kChunk, v[(c + 1) & 1]);
-                        add_scaled<C::kChunk>(sum + c * C::kChunk / 2, v[c & 1], xs + c * C::kChunk / 4);
+                        add_scaled<C::kChunk>(sum + c * C::kChunk / 2, v[c & 1], xs + c * C::kChunk / 4, sw);
                     }
                 } else {
 #pragma unroll
@@ -306,18 +289,42 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
                             uint32_t v[C::kChunk];
                             tmem_read<C::kChunk>(src + c * C::kChunk, v);
                             tmem_wait_for<C::kChunk>(v);
-                            add_scaled<C::kChunk>(sum + c * C::kChunk / 2, v, xs + c * C::kChunk / 4);
+                            add_scaled<C::kChunk>(sum + c * C::kChunk / 2, v, xs + c * C::kChunk / 4, sw);
                         }
                     }
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&sc_empty[slot]);
-                    mbar_arrive(&acc_empty[acc]);
-                }
+                if (lane == 0) mbar_arrive(&acc_empty[acc]);
                 if (++acc == (uint32_t)C::kAcc) { acc = 0; acc_ph ^= 1u; }
                 if (++slot == (uint32_t)C::kSlots) { slot = 0; slot_ph ^= 1u; }
+            }
+            if (split > 1) {
+                // Partial sums to the CTA that stores the column: rank r stores columns [r * TN / split, ..). Once every
+                // CTA of the cluster is past its last MMA (first barrier) the pipeline's stages are free to receive them,
+                // one slab per source; after the second barrier they are added in the order of the contraction.
+                const int per = TN / split, shift = __ffs(per) - 1;  // both are powers of two
+                float* slab = reinterpret_cast<float*>(smem);  // [split][per][128]
+                __syncwarp();
+                cluster_sync_all();
+                const uint32_t mine = smem_u32(slab + (size_t)rank * per * 128 + q * 32 + lane);
+#pragma unroll
+                for (int j = 0; j < C::kCols; ++j)
+                    if (j < n_tok) {
+                        const int col = col0 + j;
+                        st_cluster_f32(map_to_cta(mine + (uint32_t)(col & (per - 1)) * 512u, (uint32_t)(col >> shift)), j & 1 ? sum[j / 2].y : sum[j / 2].x);
+                    }
+                cluster_sync_all();
+                if (!ok) break;
+                const int lf = (threadIdx.x - 128) & 127, f = t.wt * 128 + lf;
+                const int n_all = n_tok + col0 - rank * per;  // live columns of this rank
+                for (int c = part; c < per && c < n_all; c += C::kEpiWarps / 4) {
+                    float total = 0.f;
+                    for (int r = 0; r < split; ++r) total += slab[((size_t)r * per + c) * 128 + lf];
+                    if (f < a.out_features)
+                        reinterpret_cast<OT*>(a.out)[(size_t)(t.row0 + rank * per + c) * a.ldo + f] = from_f32<OT>(total);
+                }
+                break;
             }
             if (!ok) break;
             const int f = t.wt * 128 + q * 32 + lane;
@@ -587,23 +594,29 @@ size_t most_tiles(const Fp8GemmArgs& a, int tokens, int features) {
     return row_tiles * (size_t)((a.out_features + features - 1) / features);
 }
 
+int launch_cluster(void (*kernel)(Fp8GemmArgs), const Fp8GemmArgs& a, unsigned grid, unsigned threads, size_t smem, unsigned cluster,
+                   cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
+}
+
 template <bool TRANS, typename OT>
 int launch_pair(const Fp8GemmArgs& a, cudaStream_t stream) {
     static bool smem_ok[kMaxDevices] = {};
     if (!allow_smem(fp8_gemm_pair_kernel<TRANS, OT>, kPairSmem, smem_ok)) return XMOE_ERR_CUDA;
     const size_t tiles = most_tiles(a, 256, 256), pairs = a.num_sms / 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles < pairs ? tiles : pairs) * 2);
-    cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = kPairSmem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel<TRANS, OT>, a) == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
+    return launch_cluster(fp8_gemm_pair_kernel<TRANS, OT>, a, (unsigned)(tiles < pairs ? tiles : pairs) * 2, kPairThreads,
+                          kPairSmem, 2, stream);
 }
 template <int TN, bool TRANS, typename OT>
 int launch_t(const Fp8GemmArgs& a, cudaStream_t stream) {
@@ -612,10 +625,13 @@ int launch_t(const Fp8GemmArgs& a, cudaStream_t stream) {
     } else {
         static bool smem_ok[kMaxDevices] = {};
         if (!allow_smem(fp8_gemm_kernel<TN, TRANS, OT>, Cfg<TN>::kSmem, smem_ok)) return XMOE_ERR_CUDA;
-        const size_t tiles = most_tiles(a, TN, 128);
-        const int grid = tiles < (size_t)a.num_sms ? (int)tiles : a.num_sms;
-        fp8_gemm_kernel<TN, TRANS, OT><<<grid, Cfg<TN>::kThreads, Cfg<TN>::kSmem, stream>>>(a);
-        return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
+        const size_t tiles = most_tiles(a, TN, 128), sms = a.num_sms;
+        Fp8GemmArgs b = a;
+        // fewer tiles than half the SMs: the contraction of a tile is shared by a cluster of 2, 4 or 8 CTAs
+        b.split = 1;
+        while (b.split < 8 && tiles * b.split * 2 <= sms && b.split * 2 * 2 <= (a.contraction + 127) / 128) b.split *= 2;
+        return launch_cluster(fp8_gemm_kernel<TN, TRANS, OT>, b, (unsigned)(tiles < sms ? tiles : sms) * b.split, Cfg<TN>::kThreads, Cfg<TN>::kSmem,
+                              b.split, stream);
     }
 }
 template <int TN>

@@ -213,6 +213,7 @@ struct Fp8GemmArgs {
     void* out;               // [rows, ldo]
     int rows, lds, ldo, mats, out_features, contraction, out_dtype, num_sms;
     int out_vec;             // out's rows are 16-byte aligned
+    int split;               // set by the launcher: CTAs that share a tile's contraction
 };
 int launch_fp8_gemm(const Fp8GemmArgs& a, int token_tile, bool transpose, cudaStream_t stream);
 int fp8_read_status(uint32_t* host_out, cudaStream_t stream);
