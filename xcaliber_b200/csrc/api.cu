@@ -1196,6 +1196,10 @@ int xmoe_unpermute(const void* rows, const int32_t* topk_row, const void* w, int
     bool empty;
     const int rc = check_permute(a, &empty);
     if (rc || empty) return rc;
+    if (k == 0 || num_rows == 0) {  // nothing comes back: y is zero
+        const size_t bytes = (size_t)n * hidden * (dtype == XMOE_FP32 ? 4 : 2);
+        return cudaMemsetAsync(y, 0, bytes, (cudaStream_t)stream) == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
+    }
     return launch_unpermute(a, (cudaStream_t)stream);
 }
 
@@ -1207,6 +1211,8 @@ int xmoe_unpermute_backward(const void* dy, const void* rows, const int32_t* top
     const int rc = check_permute(a, &empty);
     if (rc || empty || k == 0) return rc;
     if (!dw || (!drows && num_rows) || (drows && drows == rows)) return XMOE_ERR_ARG;
+    if (num_rows == 0)
+        return cudaMemsetAsync(dw, 0, (size_t)n * k * 4, (cudaStream_t)stream) == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
     return launch_unpermute_backward(a, (cudaStream_t)stream);
 }
 

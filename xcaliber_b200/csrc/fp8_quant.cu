@@ -27,61 +27,94 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
     return r;
 }
 
-// A value that rounds to e4m3 the way the exact quotient a / s does (a >= 0, s > 0, r = 1 / s rounded to nearest).
-// y = a * r with one correction by its residual is a / s to within half an fp32 step (plus 2^-47 of it), so it lies on
-// the same side of every border between two codes as a / s, or exactly on the border: borders have five significant
-// bits and are fp32 numbers. On a border (low mantissa bits as tested) the sign of the residual a - y * s, which an fma
-// gives exactly, says on which side a / s lies; y then moves one fp32 step that way.
-__device__ __forceinline__ float quotient_for_e4m3(float a, float s, float r) {
-    const float y0 = __fmul_rn(a, r);
-    const float y = __fmaf_rn(__fmaf_rn(-y0, s, a), r, y0);
+// A value that rounds to e4m3 the way the exact quotient x / s does (s > 0, r an approximation of 1 / s, off by 2^-22 of it
+// at most). y0 = x * r with one correction by its residual is x / s to within half an fp32 step and 2^-44 of it, so it
+// lies on the same side of every border between two codes as x / s, or exactly on the border: borders have at most five
+// significant bits and are fp32 numbers.
+__device__ __forceinline__ float quotient(float x, float s, float r) {
+    const float y0 = __fmul_rn(x, r);
+    return __fmaf_rn(__fmaf_rn(-y0, s, x), r, y0);
+}
+// y can only be a border if its low 19 bits are zero (normal codes: a 1 and 19 zeros below the three mantissa bits;
+// subnormal codes: odd multiples of 2^-10). Then the sign of the residual, which an fma gives exactly, says on which side
+// of the border x / s lies, and y moves one fp32 step that way.
+__device__ __forceinline__ float off_border(float y, float x, float s) {
     uint32_t bits = __float_as_uint(y);
-    // normal codes: a 1 followed by 19 zeros below the three mantissa bits; subnormal codes: odd multiples of 2^-10
-    if ((bits & 0xfffffu) == (y >= 0.015625f ? 0x80000u : 0u) && bits != 0u) {
-        const float e = __fmaf_rn(-y, s, a);
-        bits = e > 0.f ? bits + 1u : (e < 0.f ? bits - 1u : bits);
+    const float size = fabsf(y);
+    if ((bits & 0xfffffu) == (size >= 0.015625f ? 0x80000u : 0u) && size > 0.f) {
+        const float e = __fmaf_rn(-y, s, x);
+        if (e != 0.f) bits += (e > 0.f) == (y > 0.f) ? 1u : ~0u;
     }
     return __uint_as_float(bits);
 }
 
-// The block's scale from the bits of its largest magnitude, and what the lanes need to quantise with it.
-struct BlockScale {
-    float scale;        // stored
-    float s, r, shift;  // divisor, its reciprocal, power of two that keeps small blocks away from subnormal products
-    bool finite;
-};
-__device__ __forceinline__ BlockScale block_scale(uint32_t amax_bits) {
-    BlockScale b;
-    b.finite = amax_bits < 0x7f800000u;
-    b.scale = __fdiv_rn(__uint_as_float(amax_bits), kE4m3Max);
-    b.shift = b.scale < 8.6736174e-19f ? 18446744073709551616.f : 1.f;  // below 2^-60: times 2^64
-    b.s = __fmul_rn(b.scale, b.shift);
-    b.r = b.scale > 0.f ? __frcp_rn(b.s) : 0.f;
-    return b;
+__device__ __forceinline__ float max_nan(float a, float b) {  // a NaN on either side is the result
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
-// Eight values of a block, this lane's share; all 16 lanes of the block take part. Returns eight codes.
-__device__ __forceinline__ uint2 quantise8(const float* v, float& scale) {
-    uint32_t m = 0u;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);  // NaN > inf > every finite value
-#pragma unroll
-    for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const BlockScale b = block_scale(m);
-    scale = b.scale;
-    if (!b.finite) return make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+// The scale of a block from its largest magnitude, and what its lanes divide with. The usual range (all but zeros,
+// blocks below 2^-60 or above 2^120, infinities and NaN) takes the quotient by 448 as above: a / 448 is never nearer than
+// 2^-28 of itself to the middle of two fp32 numbers, so the correction rounds it correctly.
+struct BlockScale {
+    float scale, r;
+    bool usual;
+};
+__device__ __forceinline__ BlockScale block_scale(float amax) {
+    BlockScale b;
+    b.usual = amax == 0.f || (amax > 8.6736174e-19f && amax < 1.3292280e36f);
+    if (b.usual) {
+        b.scale = quotient(amax, kE4m3Max, 1.f / kE4m3Max);
+        b.r = amax == 0.f ? 0.f : rcp_approx(b.scale);
+    } else {
+        b.scale = __fdiv_rn(amax, kE4m3Max);
+        b.r = 0.f;
+    }
+    return b;
+}
+// The code of one value of an unusual block: NaN where the scale is not finite, 0 where it is 0; else divisor and value are
+// first brought to where no product is subnormal.
+__device__ __noinline__ uint32_t unusual_code(float x, float scale) {
+    if (!(scale <= 3.4028235e38f)) return 0x7fu;
+    if (scale == 0.f) return 0u;
+    const float f = scale < 1.f ? 18446744073709551616.f : 5.4210109e-20f;  // 2^64, 2^-64
+    const float s = __fmul_rn(scale, f), v = __fmul_rn(x, f);
+    return cvt_e4m3x2(off_border(quotient(v, s, __frcp_rn(s)), v, s), 0.f) & 0xffu;
+}
+
+__device__ __forceinline__ uint2 codes8(const float* v, const BlockScale& b) {
     uint32_t c[4];
+    if (b.usual) {
+        float y[8];
+        uint32_t low = ~0u;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        float y[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float x = v[2 * j + i];
-            y[i] = copysignf(quotient_for_e4m3(fabsf(x) * b.shift, b.s, b.r), x);
+        for (int j = 0; j < 8; ++j) {
+            y[j] = quotient(v[j], b.scale, b.r);
+            low = min(low, __float_as_uint(y[j]) << 13);
         }
-        c[j] = cvt_e4m3x2(y[0], y[1]);
+        if (low == 0u) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = off_border(y[j], v[j], b.scale);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = cvt_e4m3x2(y[2 * j], y[2 * j + 1]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = unusual_code(v[2 * j], b.scale) | (unusual_code(v[2 * j + 1], b.scale) << 8);
     }
     return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+}
+// Eight values of a block, this lane's share; all 16 lanes of the block take part. Returns eight codes.
+__device__ __forceinline__ uint2 quantise8(const float* v, float& scale) {
+    float m = fabsf(v[0]);
+#pragma unroll
+    for (int j = 1; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
+#pragma unroll
+    for (int d = 8; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const BlockScale b = block_scale(m);
+    scale = b.scale;
+    return codes8(v, b);
 }
 
 // Eight consecutive values of a row from column `col`, zero beyond `cols`. VEC: the row is 16-byte aligned at col.
@@ -127,31 +160,49 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int col, int cols, uin
     }
 }
 
-// How the 16 units of a CTA are laid over a row: `across` blocks of one row side by side, 16 / across rows.
-int units_across(int blocks) {
-    int a = 1;
-    while (a < kUnits && a < blocks) a *= 2;
-    return a;
-}
+// The blocks of a matrix row by row, handed out to the CTA's 16 half-warps in turn: half-warp u takes blocks u, u + 16, ..
+// of the CTA's share. Steps of 16 blocks are a fixed number of rows and blocks, so no division follows the first.
+struct Walk {
+    int row, kb;
+    __device__ __forceinline__ void step(int rows, int blocks, int kb_total) {
+        row += rows;
+        kb += blocks;
+        if (kb >= kb_total) {
+            kb -= kb_total;
+            ++row;
+        }
+    }
+};
+
+constexpr int kUnroll = 2;   // blocks per half-warp with their loads in flight together
+constexpr int kShare = 128;  // blocks per CTA of the row quantiser
 
 template <typename T, bool VEC>
-__global__ __launch_bounds__(kThreads) void fp8_quant_kernel(const Fp8QuantArgs a, int across, int kb_total) {
+__global__ __launch_bounds__(kThreads) void fp8_quant_kernel(const Fp8QuantArgs a, int kb_total, int share) {
     const int unit = threadIdx.x >> 4, l16 = threadIdx.x & 15;
-    const int rows_at_once = kUnits / across;
-    const int kb_first = blockIdx.y * across + unit % across;
     const T* x = reinterpret_cast<const T*>(a.x);
-    // every thread of a warp runs the same trip count (the shuffles need all lanes): rows and blocks past the end load
-    // nothing and store nothing
-    for (int row0 = blockIdx.x * rows_at_once; row0 < a.rows; row0 += gridDim.x * rows_at_once) {
-        const int t = row0 + unit / across;
-        for (int kb0 = 0; kb0 < kb_total; kb0 += gridDim.y * across) {
-            const int kb = kb0 + kb_first, col = kb * 128 + l16 * 8;
-            const bool on = t < a.rows && kb < kb_total;
-            float v[8];
-            load8<T, VEC>(x + (size_t)(on ? t : 0) * a.ldx, on ? col : 0, on ? a.cols : 0, v);
+    const size_t first = (size_t)blockIdx.x * share + unit;
+    Walk w{(int)(first / kb_total), (int)(first % kb_total)};
+    const int d_row = kUnits / kb_total, d_kb = kUnits % kb_total;
+    // every half-warp takes the same number of steps (the shuffles need all lanes of a warp): a block past the last row
+    // loads and stores nothing
+    for (int i = 0; i < share; i += kUnits * kUnroll) {
+        float v[kUnroll][8];
+        Walk at[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            at[u] = w;
+            if (i + u * kUnits >= share) at[u].row = a.rows;
+            const bool on = at[u].row < a.rows;
+            load8<T, VEC>(x + (size_t)(on ? at[u].row : 0) * a.ldx, on ? at[u].kb * 128 + l16 * 8 : 0, on ? a.cols : 0, v[u]);
+            w.step(d_row, d_kb, kb_total);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
             float scale;
-            const uint2 codes = quantise8(v, scale);
-            if (!on) continue;
+            const uint2 codes = quantise8(v[u], scale);
+            const int t = at[u].row, kb = at[u].kb, col = kb * 128 + l16 * 8;
+            if (t >= a.rows) continue;
             if (!a.topk_row) {
                 store_codes(a.q + (size_t)t * a.ldq, col, a.cols, codes);
                 if (l16 == 0) a.scale[(size_t)kb * a.lds + t] = scale;
@@ -167,10 +218,12 @@ __global__ __launch_bounds__(kThreads) void fp8_quant_kernel(const Fp8QuantArgs 
     }
 }
 
-// ---- gated activations: v = act(g) * u, sigmoid by expf and one reciprocal --------------------------------------------
+// ---- gated activations: v = act(g) * u ------------------------------------------------------------------------------
 // ACT 0: silu(g) * u;  1: min(g, limit) * sigmoid(alpha * min(g, limit)) * (clamp(u, -limit, limit) + 1);
 // 2: gelu_tanh(g) * u, written as g * sigmoid(2 z) (z the tanh's argument): no cancellation for negative g. NaN passes.
-__device__ __forceinline__ float sigmoid(float z) { return rcp_approx(1.f + expf(-z)); }
+// The sigmoid is 1 / (1 + 2^(-z log2 e)) with the exponential and reciprocal units (2^-22 and 2^-23 relative); the rounded
+// exponent adds |z| 2^-23.
+__device__ __forceinline__ float sigmoid(float z) { return rcp_approx(1.f + ex2_approx(z * -1.4426950408889634f)); }
 constexpr float kGeluC = 0.7978845608028654f, kGeluA = 0.044715f;
 
 template <int ACT>
@@ -205,7 +258,7 @@ __device__ __forceinline__ void glu_gradient(float g, float u, float da, float a
 // Row tiles of the live rows only: with expert segments the rows between an expert's last and the next multiple of 128
 // hold nothing and are neither read nor written.
 template <typename T, bool VEC, int ACT, bool BACKWARD>
-__global__ __launch_bounds__(kThreads) void glu_kernel(const Fp8QuantArgs a, int across, int kb_total, int tile_rows) {
+__global__ __launch_bounds__(kThreads) void glu_kernel(const Fp8QuantArgs a, int kb_total, int tile_rows) {
     __shared__ int prefix[kMaxMats + 1];
     if (a.counts) {
         if (threadIdx.x < 32) tile_prefix_build(prefix, a.counts, a.e_tot, 1, tile_rows);
@@ -213,7 +266,8 @@ __global__ __launch_bounds__(kThreads) void glu_kernel(const Fp8QuantArgs a, int
     }
     const int total = a.counts ? prefix[a.e_tot] : (a.rows + tile_rows - 1) / tile_rows;
     const int unit = threadIdx.x >> 4, l16 = threadIdx.x & 15;
-    const int rows_at_once = kUnits / across;
+    const int d_row = kUnits / kb_total, d_kb = kUnits % kb_total;
+    const Walk start{unit / kb_total, unit % kb_total};
     const T* h = reinterpret_cast<const T*>(a.x);
     for (int item = blockIdx.x; item < total; item += gridDim.x) {
         int row0 = item * tile_rows, row_end = min(row0 + tile_rows, a.rows);
@@ -223,68 +277,79 @@ __global__ __launch_bounds__(kThreads) void glu_kernel(const Fp8QuantArgs a, int
             row_end = min(row0 + min(tile_rows, t.count - t.nt_idx * tile_rows), a.rows);
             if (row0 < 0) continue;
         }
-        for (int r0 = row0; r0 < row_end; r0 += rows_at_once) {
-            const int r = r0 + unit / across;
-            for (int kb0 = blockIdx.y * across; kb0 < kb_total; kb0 += gridDim.y * across) {
-                const int kb = kb0 + unit % across, col = kb * 128 + l16 * 8;
-                const bool on = r < row_end && kb < kb_total;
-                const T* row = h + (size_t)(on ? r : row0) * a.ldx;
-                const int c = on ? col : 0, cols = on ? a.cols : 0;
-                float g[8], u[8];
-                load8<T, VEC>(row, c, cols, g);
-                load8<T, VEC>(row + a.cols, c, cols, u);
-                if (BACKWARD) {
-                    float d[8];
-                    load8<T, VEC>(reinterpret_cast<const T*>(a.da) + (size_t)(on ? r : row0) * a.cols, c, cols, d);
+        const int n_units = (row_end - row0) * kb_total;
+        Walk w = start;
+        for (int i = 0; i < n_units; i += kUnits) {
+            const int r = row0 + w.row, kb = w.kb, col = kb * 128 + l16 * 8;
+            const bool on = r < row_end;
+            w.step(d_row, d_kb, kb_total);
+            const T* row = h + (size_t)(on ? r : row0) * a.ldx;
+            const int c = on ? col : 0, cols = on ? a.cols : 0;
+            float g[8], u[8];
+            load8<T, VEC>(row, c, cols, g);
+            load8<T, VEC>(row + a.cols, c, cols, u);
+            if (BACKWARD) {
+                float d[8];
+                load8<T, VEC>(reinterpret_cast<const T*>(a.da) + (size_t)(on ? r : row0) * a.cols, c, cols, d);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) glu_gradient<ACT>(g[j], u[j], d[j], a.alpha, a.limit, g[j], u[j]);
-                    if (on) {
-                        T* out = reinterpret_cast<T*>(a.dh) + (size_t)r * 2 * a.cols;
-                        store8<T, VEC>(out, c, cols, g);
-                        store8<T, VEC>(out + a.cols, c, cols, u);
-                    }
-                } else {
+                for (int j = 0; j < 8; ++j) glu_gradient<ACT>(g[j], u[j], d[j], a.alpha, a.limit, g[j], u[j]);
+                if (on) {
+                    T* out = reinterpret_cast<T*>(a.dh) + (size_t)r * 2 * a.cols;
+                    store8<T, VEC>(out, c, cols, g);
+                    store8<T, VEC>(out + a.cols, c, cols, u);
+                }
+            } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) g[j] = col + j < cols ? glu_value<ACT>(g[j], u[j], a.alpha, a.limit) : 0.f;
-                    float scale;
-                    const uint2 codes = quantise8(g, scale);
-                    if (on) {
-                        store_codes(a.q + (size_t)r * a.ldq, col, a.cols, codes);
-                        if (l16 == 0) a.scale[(size_t)kb * a.lds + r] = scale;
-                    }
+                for (int j = 0; j < 8; ++j) g[j] = glu_value<ACT>(g[j], u[j], a.alpha, a.limit);
+                if (c + 8 > cols) {  // columns past the last take no part in the block's maximum
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) g[j] = c + j < cols ? g[j] : 0.f;
+                }
+                float scale;
+                const uint2 codes = quantise8(g, scale);
+                if (on) {
+                    store_codes(a.q + (size_t)r * a.ldq, col, a.cols, codes);
+                    if (l16 == 0) a.scale[(size_t)kb * a.lds + r] = scale;
                 }
             }
         }
     }
 }
 
-// One CTA per 128 x 128 block of a weight (load time): 64 values per thread, read twice (the second time from L2).
-template <typename T>
+// One CTA per 128 x 128 block of a weight (load time): every thread keeps eight pieces of eight values in registers.
+template <typename T, bool VEC>
 __global__ __launch_bounds__(kThreads) void fp8_quant_weight_kernel(const T* __restrict__ w, int n, int k, int nb, int kb,
                                                                     uint8_t* __restrict__ q, int ldq,
                                                                     float* __restrict__ scale) {
-    __shared__ uint32_t warp_max[kThreads / 32];
+    __shared__ float warp_max[kThreads / 32];
     const size_t block = blockIdx.x;
     const int bk = (int)(block % kb), bn = (int)(block / kb % nb);
     const size_t mat = block / kb / nb;
-    const int rows = min(128, n - bn * 128), cols = min(128, k - bk * 128);
-    const T* src = w + mat * n * k + (size_t)bn * 128 * k + (size_t)bk * 128;
-    uint32_t m = 0u;
-    for (int i = threadIdx.x; i < rows * 128; i += kThreads)
-        if ((i & 127) < cols) m = max(m, __float_as_uint(to_f32<T>(src[(size_t)(i >> 7) * k + (i & 127)])) & 0x7fffffffu);
-    m = __reduce_max_sync(0xffffffffu, m);
+    const int rows = min(128, n - bn * 128), col = bk * 128 + (threadIdx.x & 15) * 8, row = threadIdx.x >> 4;
+    const T* src = w + (mat * n + (size_t)bn * 128) * k;
+    float v[8][8], m = 0.f;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+        const int r = p * 16 + row;
+        load8<T, VEC>(src + (size_t)(r < rows ? r : 0) * k, r < rows ? col : 0, r < rows ? k : 0, v[p]);
+    }
+#pragma unroll
+    for (int p = 0; p < 8; ++p)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[p][j]));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) m = max(m, warp_max[i]);
+    for (int i = 0; i < kThreads / 32; ++i) m = max_nan(m, warp_max[i]);
     const BlockScale b = block_scale(m);
     if (threadIdx.x == 0) scale[block] = b.scale;
-    uint8_t* dst = q + mat * n * ldq + (size_t)bn * 128 * ldq + (size_t)bk * 128;
-    for (int i = threadIdx.x; i < rows * 128; i += kThreads) {
-        if ((i & 127) >= cols) continue;
-        const float x = to_f32<T>(src[(size_t)(i >> 7) * k + (i & 127)]);
-        const float y = copysignf(quotient_for_e4m3(fabsf(x) * b.shift, b.s, b.r), x);
-        dst[(size_t)(i >> 7) * ldq + (i & 127)] = b.finite ? (uint8_t)cvt_e4m3x2(y, 0.f) : (uint8_t)0x7fu;
+    uint8_t* dst = q + (mat * n + (size_t)bn * 128) * ldq;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+        const int r = p * 16 + row;
+        if (r < rows) store_codes(dst + (size_t)r * ldq, col, k, codes8(v[p], b));
     }
 }
 
@@ -293,27 +358,27 @@ bool rows_aligned(const void* p, size_t ld) { return ((uintptr_t)p & 15u) == 0 &
 
 template <typename T>
 int quant_t(const Fp8QuantArgs& a, cudaStream_t stream) {
-    const int kb = (a.cols + 127) / 128, across = units_across(kb);
-    const int row_groups = (a.rows + kUnits / across - 1) / (kUnits / across);
-    const int k_groups = (kb + across - 1) / across;
-    // few rows: the blocks of a row go to different CTAs; many rows: one CTA walks a row
-    dim3 grid(row_groups < 148 * 16 ? row_groups : 148 * 16, row_groups < 148 * 8 ? k_groups : 1);
-    if (rows_aligned<T>(a.x, a.ldx)) fp8_quant_kernel<T, true><<<grid, kThreads, 0, stream>>>(a, across, kb);
-    else fp8_quant_kernel<T, false><<<grid, kThreads, 0, stream>>>(a, across, kb);
+    const int kb = (a.cols + 127) / 128;
+    const size_t blocks = (size_t)a.rows * kb;
+    // small calls: one block per half-warp, so that every SM has some
+    const int share = blocks >= (size_t)148 * 4 * kShare ? kShare : kUnits;
+    const size_t grid = (blocks + share - 1) / share;
+    if (grid > 0x7fffffffu) return XMOE_ERR_LIMIT;
+    if (rows_aligned<T>(a.x, a.ldx)) fp8_quant_kernel<T, true><<<(unsigned)grid, kThreads, 0, stream>>>(a, kb, share);
+    else fp8_quant_kernel<T, false><<<(unsigned)grid, kThreads, 0, stream>>>(a, kb, share);
     return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
 }
 
 template <typename T, int ACT, bool BACKWARD>
 int glu_act(const Fp8QuantArgs& a, cudaStream_t stream) {
-    const int kb = (a.cols + 127) / 128, across = units_across(kb);
-    const int rows_at_once = kUnits / across;
-    const int tile_rows = rows_at_once < 4 ? 4 : rows_at_once;
+    const int kb = (a.cols + 127) / 128;
+    const int tile_rows = kb >= 4 ? 4 : 16;
     const int tiles = (a.rows + tile_rows - 1) / tile_rows;
-    const dim3 grid(tiles < 148 * 8 ? tiles : 148 * 8, 1);
+    const dim3 grid(tiles < 148 * 8 ? tiles : 148 * 8);
     const bool vec = rows_aligned<T>(a.x, a.ldx) && a.cols * sizeof(T) % 16 == 0 &&
                      (!BACKWARD || (((uintptr_t)a.da | (uintptr_t)a.dh) & 15u) == 0);
-    if (vec) glu_kernel<T, true, ACT, BACKWARD><<<grid, kThreads, 0, stream>>>(a, across, kb, tile_rows);
-    else glu_kernel<T, false, ACT, BACKWARD><<<grid, kThreads, 0, stream>>>(a, across, kb, tile_rows);
+    if (vec) glu_kernel<T, true, ACT, BACKWARD><<<grid, kThreads, 0, stream>>>(a, kb, tile_rows);
+    else glu_kernel<T, false, ACT, BACKWARD><<<grid, kThreads, 0, stream>>>(a, kb, tile_rows);
     return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
 }
 template <typename T, bool BACKWARD>
@@ -330,7 +395,8 @@ int quant_weight_t(const void* w, int mats, int n, int k, uint8_t* q, int ldq, f
     const int nb = (n + 127) / 128, kb = (k + 127) / 128;
     const size_t blocks = (size_t)mats * nb * kb;
     if (blocks > 0x7fffffffu) return XMOE_ERR_LIMIT;
-    fp8_quant_weight_kernel<T><<<(unsigned)blocks, kThreads, 0, stream>>>((const T*)w, n, k, nb, kb, q, ldq, scale);
+    if (rows_aligned<T>(w, k)) fp8_quant_weight_kernel<T, true><<<(unsigned)blocks, kThreads, 0, stream>>>((const T*)w, n, k, nb, kb, q, ldq, scale);
+    else fp8_quant_weight_kernel<T, false><<<(unsigned)blocks, kThreads, 0, stream>>>((const T*)w, n, k, nb, kb, q, ldq, scale);
     return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
 }
 

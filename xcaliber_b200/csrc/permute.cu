@@ -17,21 +17,31 @@ namespace xmoe {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSlotBatch = 8;  // rows in flight per thread
+
+// A CTA covers 256 >> shift tokens with 1 << shift threads side by side on each; blockIdx.y walks a wider row. So every
+// thread moves one vector of one token without a division, and few tokens still spread over many CTAs.
+struct Place {
+    size_t t;
+    int c;
+};
+__device__ __forceinline__ Place place(int shift) {
+    return {(size_t)blockIdx.x * (kThreads >> shift) + (threadIdx.x >> shift),
+            (int)(((size_t)blockIdx.y << shift) + (threadIdx.x & ((1 << shift) - 1)))};
+}
 
 template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void permute_kernel(const T* __restrict__ x, const int32_t* __restrict__ topk_row,
                                                            T* __restrict__ rows, int n, int hv, int k, int idx_stride,
-                                                           int num_rows) {
-    const size_t h = (size_t)hv * VEC, total = (size_t)n * hv;
-    for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (size_t)gridDim.x * kThreads) {
-        const size_t t = i / hv, c = i % hv;
-        const Pack<T, VEC> v = load_pack_once<T, VEC>(x + t * h + c * VEC);
-        const int32_t* idx = topk_row + t * idx_stride;
-        for (int s = 0; s < k; ++s) {
-            const int r = idx[s];
-            if (r >= 0 && r < num_rows) store_pack<T, VEC>(rows + (size_t)r * h + c * VEC, v);
-        }
+                                                           int num_rows, int shift) {
+    const Place p = place(shift);
+    if (p.t >= (size_t)n || p.c >= hv) return;
+    const size_t h = (size_t)hv * VEC;
+    const Pack<T, VEC> v = load_pack_once<T, VEC>(x + p.t * h + (size_t)p.c * VEC);
+    const int32_t* idx = topk_row + p.t * idx_stride;
+#pragma unroll 8
+    for (int s = 0; s < k; ++s) {
+        const int r = idx[s];
+        if (r >= 0 && r < num_rows) store_pack<T, VEC>(rows + (size_t)r * h + (size_t)p.c * VEC, v);
     }
 }
 
@@ -43,110 +53,115 @@ __device__ __forceinline__ float slot_weight(const void* w, size_t i) {
     else return 1.f;
 }
 
-template <typename T, int VEC, int WT>
+// SLOTS rows are in flight per thread. A slot without a row reads row 0 instead (so that the loads do not wait for a
+// branch each) and adds nothing.
+template <typename T, int VEC, int WT, int SLOTS>
 __global__ __launch_bounds__(kThreads) void unpermute_kernel(const T* __restrict__ rows, const int32_t* __restrict__ topk_row,
                                                              const void* __restrict__ w, T* __restrict__ y, int n, int hv,
-                                                             int k, int idx_stride, int w_stride, int num_rows) {
-    const size_t h = (size_t)hv * VEC, total = (size_t)n * hv;
-    for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (size_t)gridDim.x * kThreads) {
-        const size_t t = i / hv, c = i % hv;
-        const int32_t* idx = topk_row + t * idx_stride;
-        float acc[VEC];
+                                                             int k, int idx_stride, int w_stride, int num_rows, int shift) {
+    const Place p = place(shift);
+    if (p.t >= (size_t)n || p.c >= hv) return;
+    const size_t h = (size_t)hv * VEC;
+    const int32_t* idx = topk_row + p.t * idx_stride;
+    float acc[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-        for (int s0 = 0; s0 < k; s0 += kSlotBatch) {
-            Pack<T, VEC> v[kSlotBatch];
-            float ws[kSlotBatch];
-            bool on[kSlotBatch];
+    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    for (int s0 = 0; s0 < k; s0 += SLOTS) {
+        int r[SLOTS];
+        Pack<T, VEC> v[SLOTS];
+        float ws[SLOTS];
 #pragma unroll
-            for (int s = 0; s < kSlotBatch; ++s) {
-                const int r = s0 + s < k ? idx[s0 + s] : -1;
-                on[s] = r >= 0 && r < num_rows;
-                if (on[s]) {
-                    v[s] = load_pack_once<T, VEC>(rows + (size_t)r * h + c * VEC);
-                    ws[s] = slot_weight<WT>(w, t * w_stride + s0 + s);
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < kSlotBatch; ++s)
-                if (on[s]) {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        acc[j] = WT ? fmaf(ws[s], to_f32<T>(v[s].v[j]), acc[j]) : acc[j] + to_f32<T>(v[s].v[j]);
-                }
+        for (int s = 0; s < SLOTS; ++s) {
+            r[s] = s0 + s < k ? idx[s0 + s] : -1;
+            if (r[s] >= num_rows) r[s] = -1;
+            ws[s] = slot_weight<WT>(w, p.t * w_stride + min(s0 + s, k - 1));
         }
-        Pack<T, VEC> o;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) o.v[j] = from_f32<T>(acc[j]);
-        store_pack<T, VEC>(y + t * h + c * VEC, o);
+        for (int s = 0; s < SLOTS; ++s) v[s] = load_pack_once<T, VEC>(rows + (size_t)max(r[s], 0) * h + (size_t)p.c * VEC);
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float x = to_f32<T>(v[s].v[j]);
+                acc[j] = r[s] < 0 ? acc[j] : (WT ? fmaf(ws[s], x, acc[j]) : acc[j] + x);
+            }
     }
+    Pack<T, VEC> o;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) o.v[j] = from_f32<T>(acc[j]);
+    store_pack<T, VEC>(y + p.t * h + (size_t)p.c * VEC, o);
 }
 
 // One CTA per token: dy[t] is read once per batch of slots, every thread keeps one partial dot product per slot, and
 // the partials are added over the warp and then over the warps in a fixed order.
-template <typename T, int VEC, int WT>
+template <typename T, int VEC, int WT, int SLOTS>
 __global__ __launch_bounds__(kThreads) void unpermute_backward_kernel(const T* __restrict__ dy, const T* __restrict__ rows,
                                                                       const int32_t* __restrict__ topk_row,
                                                                       const void* __restrict__ w, T* __restrict__ drows,
                                                                       float* __restrict__ dw, int n, int hv, int k,
                                                                       int idx_stride, int w_stride, int num_rows) {
-    __shared__ float part[kThreads / 32][kSlotBatch];
+    __shared__ float part[kThreads / 32][SLOTS];
     const size_t h = (size_t)hv * VEC;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (size_t t = blockIdx.x; t < (size_t)n; t += gridDim.x) {
-        for (int s0 = 0; s0 < k; s0 += kSlotBatch) {
-            int r[kSlotBatch];
-            float ws[kSlotBatch], dot[kSlotBatch];
+        for (int s0 = 0; s0 < k; s0 += SLOTS) {
+            int r[SLOTS];
+            float ws[SLOTS], dot[SLOTS];
 #pragma unroll
-            for (int s = 0; s < kSlotBatch; ++s) {
+            for (int s = 0; s < SLOTS; ++s) {
                 r[s] = s0 + s < k ? topk_row[t * idx_stride + s0 + s] : -1;
                 if (r[s] >= num_rows) r[s] = -1;
-                ws[s] = r[s] >= 0 ? slot_weight<WT>(w, t * w_stride + s0 + s) : 0.f;
+                ws[s] = slot_weight<WT>(w, t * w_stride + min(s0 + s, k - 1));
                 dot[s] = 0.f;
             }
             for (int c = threadIdx.x; c < hv; c += kThreads) {
                 const Pack<T, VEC> g = load_pack<T, VEC>(dy + t * h + (size_t)c * VEC);
+                Pack<T, VEC> v[SLOTS];
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s) v[s] = load_pack_once<T, VEC>(rows + (size_t)max(r[s], 0) * h + (size_t)c * VEC);
                 float gf[VEC];
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) gf[j] = to_f32<T>(g.v[j]);
-                Pack<T, VEC> v[kSlotBatch];
 #pragma unroll
-                for (int s = 0; s < kSlotBatch; ++s)
-                    if (r[s] >= 0) v[s] = load_pack_once<T, VEC>(rows + (size_t)r[s] * h + (size_t)c * VEC);
+                for (int s = 0; s < SLOTS; ++s) {
+                    Pack<T, VEC> o;
 #pragma unroll
-                for (int s = 0; s < kSlotBatch; ++s)
-                    if (r[s] >= 0) {
-                        Pack<T, VEC> o;
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) {
-                            dot[s] = fmaf(gf[j], to_f32<T>(v[s].v[j]), dot[s]);
-                            o.v[j] = from_f32<T>(ws[s] * gf[j]);
-                        }
-                        store_pack<T, VEC>(drows + (size_t)r[s] * h + (size_t)c * VEC, o);
+                    for (int j = 0; j < VEC; ++j) {
+                        dot[s] = fmaf(gf[j], to_f32<T>(v[s].v[j]), dot[s]);
+                        o.v[j] = from_f32<T>(ws[s] * gf[j]);
                     }
+                    if (r[s] >= 0) store_pack<T, VEC>(drows + (size_t)r[s] * h + (size_t)c * VEC, o);
+                }
             }
 #pragma unroll
-            for (int s = 0; s < kSlotBatch; ++s) {
+            for (int s = 0; s < SLOTS; ++s) {
 #pragma unroll
                 for (int d = 16; d; d >>= 1) dot[s] += __shfl_xor_sync(0xffffffffu, dot[s], d);
-                if (lane == 0) part[warp][s] = dot[s];
+                if (lane == 0) part[warp][s] = r[s] < 0 ? 0.f : dot[s];
             }
             __syncthreads();
-            if (threadIdx.x < kSlotBatch && s0 + (int)threadIdx.x < k) {
+            if (threadIdx.x < SLOTS && s0 + (int)threadIdx.x < k) {
                 float sum = 0.f;
 #pragma unroll
                 for (int q = 0; q < kThreads / 32; ++q) sum += part[q][threadIdx.x];
-                dw[t * k + s0 + threadIdx.x] = sum;  // a slot without a row: its partials are all zero
+                dw[t * k + s0 + threadIdx.x] = sum;
             }
             __syncthreads();
         }
     }
 }
 
-int grid_for(size_t threads) {
-    const size_t blocks = (threads + kThreads - 1) / kThreads;
-    return (int)(blocks < 148 * 32 ? blocks : 148 * 32);
+// Threads side by side on a row: the power of two that covers it, 32 to 256.
+int row_shift(int hv) {
+    int shift = 5;
+    while (shift < 8 && (1 << shift) < hv) ++shift;
+    return shift;
 }
+dim3 grid_for(int n, int hv, int shift) {
+    const int tokens = kThreads >> shift;
+    return dim3((unsigned)((n + (size_t)tokens - 1) / tokens), (unsigned)((hv + (1ll << shift) - 1) >> shift));
+}
+constexpr int kMaxGridY = 65535;
 
 template <typename T>
 bool vectors_ok(int h, const void* a, const void* b, const void* c) {
@@ -154,43 +169,52 @@ bool vectors_ok(int h, const void* a, const void* b, const void* c) {
            (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15u) == 0;
 }
 
-template <typename T>
-int permute_t(const PermuteArgs& a, cudaStream_t stream) {
-    constexpr int V = 16 / sizeof(T);
-    if (vectors_ok<T>(a.H, a.x, a.rows, nullptr))
-        permute_kernel<T, V><<<grid_for((size_t)a.N * (a.H / V)), kThreads, 0, stream>>>(
-            (const T*)a.x, a.topk_row, (T*)a.rows, a.N, a.H / V, a.k, a.idx_stride, a.num_rows);
-    else
-        permute_kernel<T, 1><<<grid_for((size_t)a.N * a.H), kThreads, 0, stream>>>((const T*)a.x, a.topk_row, (T*)a.rows, a.N,
-                                                                                   a.H, a.k, a.idx_stride, a.num_rows);
+template <typename T, int V>
+int permute_v(const PermuteArgs& a, cudaStream_t stream) {
+    const int hv = a.H / V, shift = row_shift(hv);
+    const dim3 grid = grid_for(a.N, hv, shift);
+    if (grid.y > kMaxGridY) return XMOE_ERR_LIMIT;
+    permute_kernel<T, V><<<grid, kThreads, 0, stream>>>((const T*)a.x, a.topk_row, (T*)a.rows, a.N, hv, a.k, a.idx_stride,
+                                                        a.num_rows, shift);
     return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
 }
+template <typename T>
+int permute_t(const PermuteArgs& a, cudaStream_t stream) {
+    if (vectors_ok<T>(a.H, a.x, a.rows, nullptr)) return permute_v<T, 16 / sizeof(T)>(a, stream);
+    return permute_v<T, 1>(a, stream);
+}
 
+template <typename T, int V, int WT, int SLOTS>
+int unpermute_s(const PermuteArgs& a, cudaStream_t stream) {
+    const int hv = a.H / V, shift = row_shift(hv);
+    const dim3 grid = grid_for(a.N, hv, shift);
+    if (grid.y > kMaxGridY) return XMOE_ERR_LIMIT;
+    unpermute_kernel<T, V, WT, SLOTS><<<grid, kThreads, 0, stream>>>((const T*)a.rows, a.topk_row, a.w, (T*)a.x, a.N, hv, a.k,
+                                                                     a.idx_stride, a.w_stride, a.num_rows, shift);
+    return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
+}
+template <typename T, int V, int WT, int SLOTS>
+int unpermute_backward_s(const PermuteArgs& a, cudaStream_t stream) {
+    const int grid = a.N < 148 * 64 ? a.N : 148 * 64;
+    unpermute_backward_kernel<T, V, WT, SLOTS><<<grid, kThreads, 0, stream>>>((const T*)a.x, (const T*)a.rows, a.topk_row, a.w,
+                                                                              (T*)a.drows, a.dw, a.N, a.H / V, a.k,
+                                                                              a.idx_stride, a.w_stride, a.num_rows);
+    return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
+}
+// rows in flight per thread: the smallest of 2, 4, 8 that holds a token's slots
+#define XMOE_BY_SLOTS(fn, T, V, WT) \
+    (a.k <= 2 ? fn<T, V, WT, 2>(a, stream) : a.k <= 4 ? fn<T, V, WT, 4>(a, stream) : fn<T, V, WT, 8>(a, stream))
 template <typename T, int WT>
 int unpermute_t(const PermuteArgs& a, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
-    if (vectors_ok<T>(a.H, a.x, a.rows, nullptr))
-        unpermute_kernel<T, V, WT><<<grid_for((size_t)a.N * (a.H / V)), kThreads, 0, stream>>>(
-            (const T*)a.rows, a.topk_row, a.w, (T*)a.x, a.N, a.H / V, a.k, a.idx_stride, a.w_stride, a.num_rows);
-    else
-        unpermute_kernel<T, 1, WT><<<grid_for((size_t)a.N * a.H), kThreads, 0, stream>>>(
-            (const T*)a.rows, a.topk_row, a.w, (T*)a.x, a.N, a.H, a.k, a.idx_stride, a.w_stride, a.num_rows);
-    return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
+    if (vectors_ok<T>(a.H, a.x, a.rows, nullptr)) return XMOE_BY_SLOTS(unpermute_s, T, V, WT);
+    return XMOE_BY_SLOTS(unpermute_s, T, 1, WT);
 }
-
 template <typename T, int WT>
 int unpermute_backward_t(const PermuteArgs& a, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
-    const int grid = a.N < 148 * 64 ? a.N : 148 * 64;
-    if (vectors_ok<T>(a.H, a.x, a.rows, a.drows))
-        unpermute_backward_kernel<T, V, WT><<<grid, kThreads, 0, stream>>>((const T*)a.x, (const T*)a.rows, a.topk_row, a.w,
-                                                                           (T*)a.drows, a.dw, a.N, a.H / V, a.k, a.idx_stride,
-                                                                           a.w_stride, a.num_rows);
-    else
-        unpermute_backward_kernel<T, 1, WT><<<grid, kThreads, 0, stream>>>((const T*)a.x, (const T*)a.rows, a.topk_row, a.w,
-                                                                           (T*)a.drows, a.dw, a.N, a.H, a.k, a.idx_stride,
-                                                                           a.w_stride, a.num_rows);
-    return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
+    if (vectors_ok<T>(a.H, a.x, a.rows, a.drows)) return XMOE_BY_SLOTS(unpermute_backward_s, T, V, WT);
+    return XMOE_BY_SLOTS(unpermute_backward_s, T, 1, WT);
 }
 
 #define XMOE_BY_WEIGHT(fn, T)                     \
