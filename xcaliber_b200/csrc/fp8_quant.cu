@@ -5,8 +5,8 @@
 // A block of zeros (or one whose scale underflows) has scale 0 and zero codes; a block that holds an infinity or a NaN
 // has the scale max|v| / 448 = inf or NaN and NaN codes, so that whatever is computed from it shows it.
 //
-// One block of 128 is handled by 16 lanes with 8 values each: a 16-byte load per lane (bf16, fp16), four shuffles for
-// the maximum, an 8-byte store. Scales are stored block-major, [ceil(cols / 128), lds], the order in which the product
+// One block of 128 is handled by 8 lanes with twice 8 values each: two coalesced 16-byte loads per lane (bf16, fp16), three
+// shuffles for the maximum, two 8-byte stores. Scales are stored block-major, [ceil(cols / 128), lds], the order in which the product
 // reads them: the scales of consecutive rows for one block are contiguous.
 #include "elem.cuh"
 #include "kernels.h"
@@ -17,7 +17,8 @@ namespace xmoe {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnits = kThreads / 16;  // 128-value blocks a CTA handles at once
+constexpr int kLanes = 8;                  // per block of 128 values
+constexpr int kUnits = kThreads / kLanes;  // blocks a CTA handles at once
 constexpr int kMaxMats = 1032;
 constexpr float kE4m3Max = 448.f;
 
@@ -27,27 +28,12 @@ __device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
     return r;
 }
 
-// A value that rounds to e4m3 the way the exact quotient x / s does (s > 0, r an approximation of 1 / s, off by 2^-22 of it
-// at most). y0 = x * r with one correction by its residual is x / s to within half an fp32 step and 2^-44 of it, so it
-// lies on the same side of every border between two codes as x / s, or exactly on the border: borders have at most five
-// significant bits and are fp32 numbers.
+// x / s to within half an fp32 step and 2^-44 of it (s > 0, r an approximation of 1 / s, off by 2^-22 of it at most): the
+// product with r, corrected once by its residual.
 __device__ __forceinline__ float quotient(float x, float s, float r) {
     const float y0 = __fmul_rn(x, r);
     return __fmaf_rn(__fmaf_rn(-y0, s, x), r, y0);
 }
-// y can only be a border if its low 19 bits are zero (normal codes: a 1 and 19 zeros below the three mantissa bits;
-// subnormal codes: odd multiples of 2^-10). Then the sign of the residual, which an fma gives exactly, says on which side
-// of the border x / s lies, and y moves one fp32 step that way.
-__device__ __forceinline__ float off_border(float y, float x, float s) {
-    uint32_t bits = __float_as_uint(y);
-    const float size = fabsf(y);
-    if ((bits & 0xfffffu) == (size >= 0.015625f ? 0x80000u : 0u) && size > 0.f) {
-        const float e = __fmaf_rn(-y, s, x);
-        if (e != 0.f) bits += (e > 0.f) == (y > 0.f) ? 1u : ~0u;
-    }
-    return __uint_as_float(bits);
-}
-
 __device__ __forceinline__ float max_nan(float a, float b) {  // a NaN on either side is the result
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -73,65 +59,106 @@ __device__ __forceinline__ BlockScale block_scale(float amax) {
     }
     return b;
 }
-// The code of one value of an unusual block: NaN where the scale is not finite, 0 where it is 0; else divisor and value are
-// first brought to where no product is subnormal.
-__device__ __noinline__ uint32_t unusual_code(float x, float scale) {
-    if (!(scale <= 3.4028235e38f)) return 0x7fu;
+// Two neighbouring codes of which the exact x / s rounds to one, in byte j of lo and hi: the sign of x - T s, with T the
+// border between them (the middle of two code values is an fp32 number, and an fma gives the sign exactly), says on
+// which side it lies; on the border itself the even code is the one.
+__device__ __forceinline__ uint32_t decide(uint32_t lo, uint32_t hi, float x, float s) {
+    uint32_t both;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(both) : "h"((uint16_t)(lo | (hi << 8))));
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&both));
+    const float side = copysignf(1.f, x) * __fmaf_rn(-0.5f * (v.x + v.y), s, x);
+    return side > 0.f || (side == 0.f && (lo & 1u)) ? hi : lo;
+}
+
+// Codes of N values x / s, r approximating 1 / s to 2^-23 of it. Two products bracket every quotient (the factors move
+// r by 2^-21, each product adds 2^-24): where both round to the same code, so does the quotient. They differ only next to
+// a border: rarely for fp32 values, more often where values and scale have few bits (bf16), so that is cheap too.
+template <int N>
+__device__ __forceinline__ void bracket(const float* v, float s, float r, uint32_t* code) {
+    const float r_lo = r * (1.f - 4.7683716e-7f), r_hi = r * (1.f + 4.7683716e-7f);
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+        const float* x = v + 4 * j;
+        code[j] = cvt_e4m3x2(x[0] * r_lo, x[1] * r_lo) | (cvt_e4m3x2(x[2] * r_lo, x[3] * r_lo) << 16);
+        const uint32_t hi = cvt_e4m3x2(x[0] * r_hi, x[1] * r_hi) | (cvt_e4m3x2(x[2] * r_hi, x[3] * r_hi) << 16);
+        if (code[j] != hi) {
+            const uint32_t lo = code[j];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t l = (lo >> (8 * i)) & 0xffu, h = (hi >> (8 * i)) & 0xffu;
+                if (l != h) code[j] ^= (l ^ decide(l, h, x[i], s)) << (8 * i);
+            }
+        }
+    }
+}
+// An unusual block: NaN codes where the scale is not finite, 0 where it is 0; else divisor and values are first brought to
+// where no product is subnormal.
+__device__ __noinline__ uint32_t unusual4(float4 a, float scale) {
+    if (!(scale <= 3.4028235e38f)) return 0x7f7f7f7fu;
     if (scale == 0.f) return 0u;
     const float f = scale < 1.f ? 18446744073709551616.f : 5.4210109e-20f;  // 2^64, 2^-64
-    const float s = __fmul_rn(scale, f), v = __fmul_rn(x, f);
-    return cvt_e4m3x2(off_border(quotient(v, s, __frcp_rn(s)), v, s), 0.f) & 0xffu;
+    const float v[4] = {a.x * f, a.y * f, a.z * f, a.w * f}, s = scale * f;
+    uint32_t code;
+    bracket<4>(v, s, __frcp_rn(s), &code);
+    return code;
 }
-
-__device__ __forceinline__ uint2 codes8(const float* v, const BlockScale& b) {
-    uint32_t c[4];
+// N is 8 times the pieces a lane holds
+template <int N>
+__device__ __forceinline__ void codes_of(const float* v, const BlockScale& b, uint32_t* code) {
     if (b.usual) {
-        float y[8];
-        uint32_t low = ~0u;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            y[j] = quotient(v[j], b.scale, b.r);
-            low = min(low, __float_as_uint(y[j]) << 13);
-        }
-        if (low == 0u) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = off_border(y[j], v[j], b.scale);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c[j] = cvt_e4m3x2(y[2 * j], y[2 * j + 1]);
+        bracket<N>(v, b.scale, b.r, code);
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c[j] = unusual_code(v[2 * j], b.scale) | (unusual_code(v[2 * j + 1], b.scale) << 8);
+        for (int j = 0; j < N / 4; ++j) code[j] = unusual4(make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]), b.scale);
     }
-    return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
 }
-// Eight values of a block, this lane's share; all 16 lanes of the block take part. Returns eight codes.
-__device__ __forceinline__ uint2 quantise8(const float* v, float& scale) {
-    float m = fabsf(v[0]);
+// Sixteen values of a block, this lane's share, `m` their largest magnitude; all lanes of the block take part.
+__device__ __forceinline__ void quantise16(const float* v, float m, uint32_t* code, float& scale) {
 #pragma unroll
-    for (int j = 1; j < 8; ++j) m = max_nan(m, fabsf(v[j]));
-#pragma unroll
-    for (int d = 8; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+    for (int d = kLanes / 2; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
     const BlockScale b = block_scale(m);
     scale = b.scale;
-    return codes8(v, b);
+    codes_of<16>(v, b, code);
+}
+template <int N>
+__device__ __forceinline__ float largest(const float* v) {
+    float m = fabsf(v[0]);
+#pragma unroll
+    for (int j = 1; j < N; ++j) m = max_nan(m, fabsf(v[j]));
+    return m;
 }
 
-// Eight consecutive values of a row from column `col`, zero beyond `cols`. VEC: the row is 16-byte aligned at col.
+// The largest magnitude of the eight values of a 16-byte piece of 16-bit values, two at a time (a NaN is the result).
+__device__ __forceinline__ float largest8(const Pack<__nv_bfloat16, 8>& k) {
+    const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&k);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
+    return max_nan(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float largest8(const Pack<__half, 8>& k) {
+    const __half2* p = reinterpret_cast<const __half2*>(&k);
+    const __half2 m = __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
+    return max_nan(__low2float(m), __high2float(m));
+}
+// Eight consecutive values of a row from column `col`, zero beyond `cols`, and their largest magnitude. VEC: the row is
+// 16-byte aligned at col.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int col, int cols, float* v) {
+__device__ __forceinline__ float load8(const T* row, int col, int cols, float* v) {
     if (VEC && col + 8 <= cols) {
         constexpr int P = 16 / sizeof(T);
+        float m = 0.f;
 #pragma unroll
         for (int p = 0; p < 8 / P; ++p) {
             const Pack<T, P> k = load_pack_once<T, P>(row + col + p * P);
 #pragma unroll
             for (int j = 0; j < P; ++j) v[p * P + j] = to_f32<T>(k.v[j]);
+            if constexpr (P == 8) m = largest8(k);
+            else m = max_nan(m, largest<P>(v + p * P));
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = col + j < cols ? to_f32<T>(row[col + j]) : 0.f;
+        return m;
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = col + j < cols ? to_f32<T>(row[col + j]) : 0.f;
+    return largest<8>(v);
 }
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(T* row, int col, int cols, const float* v) {
@@ -151,17 +178,17 @@ __device__ __forceinline__ void store8(T* row, int col, int cols, const float* v
     }
 }
 // code rows start at multiples of 16 bytes, so eight codes from a multiple of 8 are one aligned store
-__device__ __forceinline__ void store_codes(uint8_t* row, int col, int cols, uint2 c) {
+__device__ __forceinline__ void store_codes(uint8_t* row, int col, int cols, const uint32_t* c) {
     if (col + 8 <= cols) {
-        *reinterpret_cast<uint2*>(row + col) = c;
+        *reinterpret_cast<uint2*>(row + col) = make_uint2(c[0], c[1]);
     } else {
-        const unsigned long long w = ((unsigned long long)c.y << 32) | c.x;
+        const unsigned long long w = ((unsigned long long)c[1] << 32) | c[0];
         for (int j = 0; col + j < cols; ++j) row[col + j] = (uint8_t)(w >> (8 * j));
     }
 }
 
-// The blocks of a matrix row by row, handed out to the CTA's 16 half-warps in turn: half-warp u takes blocks u, u + 16, ..
-// of the CTA's share. Steps of 16 blocks are a fixed number of rows and blocks, so no division follows the first.
+// The blocks of a matrix row by row, handed out to the CTA's kUnits groups of lanes in turn: group u takes blocks u, u +
+// kUnits, .. of the CTA's share. Steps of kUnits blocks are a fixed number of rows and blocks: no division follows the first.
 struct Walk {
     int row, kb;
     __device__ __forceinline__ void step(int rows, int blocks, int kb_total) {
@@ -174,46 +201,33 @@ struct Walk {
     }
 };
 
-constexpr int kUnroll = 2;   // blocks per half-warp with their loads in flight together
-constexpr int kShare = 128;  // blocks per CTA of the row quantiser
-
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool SORTED>
 __global__ __launch_bounds__(kThreads) void fp8_quant_kernel(const Fp8QuantArgs a, int kb_total, int share) {
-    const int unit = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+    const int unit = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
     const T* x = reinterpret_cast<const T*>(a.x);
     const size_t first = (size_t)blockIdx.x * share + unit;
     Walk w{(int)(first / kb_total), (int)(first % kb_total)};
     const int d_row = kUnits / kb_total, d_kb = kUnits % kb_total;
-    // every half-warp takes the same number of steps (the shuffles need all lanes of a warp): a block past the last row
-    // loads and stores nothing
-    for (int i = 0; i < share; i += kUnits * kUnroll) {
-        float v[kUnroll][8];
-        Walk at[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            at[u] = w;
-            if (i + u * kUnits >= share) at[u].row = a.rows;
-            const bool on = at[u].row < a.rows;
-            load8<T, VEC>(x + (size_t)(on ? at[u].row : 0) * a.ldx, on ? at[u].kb * 128 + l16 * 8 : 0, on ? a.cols : 0, v[u]);
-            w.step(d_row, d_kb, kb_total);
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            float scale;
-            const uint2 codes = quantise8(v[u], scale);
-            const int t = at[u].row, kb = at[u].kb, col = kb * 128 + l16 * 8;
-            if (t >= a.rows) continue;
-            if (!a.topk_row) {
-                store_codes(a.q + (size_t)t * a.ldq, col, a.cols, codes);
-                if (l16 == 0) a.scale[(size_t)kb * a.lds + t] = scale;
-            } else {
-                for (int s = 0; s < a.k; ++s) {
-                    const int r = a.topk_row[(size_t)t * a.idx_stride + s];
-                    if (r < 0 || r >= a.num_rows) continue;
-                    store_codes(a.q + (size_t)r * a.ldq, col, a.cols, codes);
-                    if (l16 == 0) a.scale[(size_t)kb * a.lds + r] = scale;
-                }
-            }
+    // every group takes the same number of steps (the shuffles need all lanes of a warp): a block past the last row loads
+    // and stores nothing
+    for (int i = 0; i < share; i += kUnits, w.step(d_row, d_kb, kb_total)) {
+        const int t = w.row, kb = w.kb, col = kb * 128 + lane * 8;
+        const bool on = t < a.rows;
+        const T* row = x + (size_t)(on ? t : 0) * a.ldx;
+        const int cols = on ? a.cols : 0;
+        float v[16];
+        const float m = max_nan(load8<T, VEC>(row, col, cols, v), load8<T, VEC>(row, col + 64, cols, v + 8));
+        uint32_t code[4];
+        float scale;
+        quantise16(v, m, code, scale);
+        if (!on) continue;
+        for (int s = 0; s < (SORTED ? a.k : 1); ++s) {
+            const int r = SORTED ? a.topk_row[(size_t)t * a.idx_stride + s] : t;
+            if (SORTED && (r < 0 || r >= a.num_rows)) continue;
+            uint8_t* q = a.q + (size_t)r * a.ldq;
+            store_codes(q, col, a.cols, code);
+            store_codes(q, col + 64, a.cols, code + 2);
+            if (lane == 0) a.scale[(size_t)kb * a.lds + r] = scale;
         }
     }
 }
@@ -255,62 +269,76 @@ __device__ __forceinline__ void glu_gradient(float g, float u, float da, float a
     }
 }
 
-// Row tiles of the live rows only: with expert segments the rows between an expert's last and the next multiple of 128
-// hold nothing and are neither read nor written.
+// Live rows only: with expert segments the rows between an expert's last and the next multiple of 128 hold nothing and are
+// neither read nor written. The live rows are numbered through; every CTA takes an equal, contiguous share of their blocks
+// and finds its first expert once.
 template <typename T, bool VEC, int ACT, bool BACKWARD>
-__global__ __launch_bounds__(kThreads) void glu_kernel(const Fp8QuantArgs a, int kb_total, int tile_rows) {
-    __shared__ int prefix[kMaxMats + 1];
+__global__ __launch_bounds__(kThreads, BACKWARD ? 1 : 4) void glu_kernel(const Fp8QuantArgs a, int kb_total) {
+    // the gradient has no block to share a scale: 16 lanes with 8 values, for more warps in flight
+    constexpr int kP = BACKWARD ? 1 : 2, kLanes = 16 / kP, kUnits = kThreads / kLanes;
+    __shared__ int before[kMaxMats + 1];  // live rows of the experts before e
+    __shared__ int shift[kMaxMats];       // buffer row - live row, within expert e
+    const int mats = a.counts ? a.e_tot : 1;
     if (a.counts) {
-        if (threadIdx.x < 32) tile_prefix_build(prefix, a.counts, a.e_tot, 1, tile_rows);
-        __syncthreads();
+        if (threadIdx.x < 32) tile_prefix_build(before, a.counts, mats, 1, 1);
+    } else if (threadIdx.x == 0) {
+        before[0] = 0;
+        before[1] = a.rows;
     }
-    const int total = a.counts ? prefix[a.e_tot] : (a.rows + tile_rows - 1) / tile_rows;
-    const int unit = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+    __syncthreads();
+    for (int e = threadIdx.x; e < mats; e += kThreads) shift[e] = (a.counts ? a.offsets[e] : 0) - before[e];
+    __syncthreads();
+    const int live = before[mats];
+    const size_t blocks = (size_t)live * kb_total;
+    const size_t share = ((blocks + gridDim.x - 1) / gridDim.x + kUnits - 1) / kUnits * kUnits;
+    const size_t begin = blockIdx.x * share;
+    if (begin >= blocks) return;
+    const int steps = (int)(((begin + share < blocks ? share : blocks - begin) + kUnits - 1) / kUnits);
+    const int unit = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+    Walk w{(int)((begin + unit) / kb_total), (int)((begin + unit) % kb_total)};
     const int d_row = kUnits / kb_total, d_kb = kUnits % kb_total;
-    const Walk start{unit / kb_total, unit % kb_total};
+    int e = 0;
+    for (int hi = mats; hi - e > 1;) {  // largest e with before[e] <= row
+        const int mid = (e + hi) >> 1;
+        if (before[mid] <= w.row) e = mid; else hi = mid;
+    }
     const T* h = reinterpret_cast<const T*>(a.x);
-    for (int item = blockIdx.x; item < total; item += gridDim.x) {
-        int row0 = item * tile_rows, row_end = min(row0 + tile_rows, a.rows);
-        if (a.counts) {
-            const TileInfo t = tile_decode(item, prefix, a.counts, a.offsets, a.e_tot, tile_rows);
-            row0 = t.row0;
-            row_end = min(row0 + min(tile_rows, t.count - t.nt_idx * tile_rows), a.rows);
-            if (row0 < 0) continue;
+    for (int i = 0; i < steps; ++i, w.step(d_row, d_kb, kb_total)) {
+        while (e + 1 < mats && before[e + 1] <= w.row) ++e;
+        const int r = w.row + shift[e], kb = w.kb, col = kb * 128 + lane * 8;
+        const bool on = w.row < live && r >= 0 && r < a.rows;
+        const size_t at = on ? r : 0;
+        const int cols = on ? a.cols : 0;
+        const T* row = h + at * a.ldx;
+        float g[8 * kP], u[8 * kP];
+#pragma unroll
+        for (int p = 0; p < kP; ++p) {
+            load8<T, VEC>(row, col + p * 64, cols, g + 8 * p);
+            load8<T, VEC>(row + a.cols, col + p * 64, cols, u + 8 * p);
         }
-        const int n_units = (row_end - row0) * kb_total;
-        Walk w = start;
-        for (int i = 0; i < n_units; i += kUnits) {
-            const int r = row0 + w.row, kb = w.kb, col = kb * 128 + l16 * 8;
-            const bool on = r < row_end;
-            w.step(d_row, d_kb, kb_total);
-            const T* row = h + (size_t)(on ? r : row0) * a.ldx;
-            const int c = on ? col : 0, cols = on ? a.cols : 0;
-            float g[8], u[8];
-            load8<T, VEC>(row, c, cols, g);
-            load8<T, VEC>(row + a.cols, c, cols, u);
-            if (BACKWARD) {
-                float d[8];
-                load8<T, VEC>(reinterpret_cast<const T*>(a.da) + (size_t)(on ? r : row0) * a.cols, c, cols, d);
+        if constexpr (BACKWARD) {
+            float d[8];
+            load8<T, VEC>(reinterpret_cast<const T*>(a.da) + at * a.cols, col, cols, d);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) glu_gradient<ACT>(g[j], u[j], d[j], a.alpha, a.limit, g[j], u[j]);
-                if (on) {
-                    T* out = reinterpret_cast<T*>(a.dh) + (size_t)r * 2 * a.cols;
-                    store8<T, VEC>(out, c, cols, g);
-                    store8<T, VEC>(out + a.cols, c, cols, u);
-                }
-            } else {
+            for (int j = 0; j < 8; ++j) glu_gradient<ACT>(g[j], u[j], d[j], a.alpha, a.limit, g[j], u[j]);
+            T* out = reinterpret_cast<T*>(a.dh) + at * 2 * a.cols;
+            store8<T, VEC>(out, col, cols, g);
+            store8<T, VEC>(out + a.cols, col, cols, u);
+        } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] = glu_value<ACT>(g[j], u[j], a.alpha, a.limit);
-                if (c + 8 > cols) {  // columns past the last take no part in the block's maximum
+            for (int j = 0; j < 16; ++j) g[j] = glu_value<ACT>(g[j], u[j], a.alpha, a.limit);
+            if (col + 72 > cols) {  // columns past the last take no part in the block's maximum
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) g[j] = c + j < cols ? g[j] : 0.f;
-                }
-                float scale;
-                const uint2 codes = quantise8(g, scale);
-                if (on) {
-                    store_codes(a.q + (size_t)r * a.ldq, col, a.cols, codes);
-                    if (l16 == 0) a.scale[(size_t)kb * a.lds + r] = scale;
-                }
+                for (int j = 0; j < 16; ++j) g[j] = col + (j < 8 ? j : j + 56) < cols ? g[j] : 0.f;
+            }
+            uint32_t code[4];
+            float scale;
+            quantise16(g, largest<16>(g), code, scale);
+            if (on) {
+                uint8_t* q = a.q + at * a.ldq;
+                store_codes(q, col, cols, code);
+                store_codes(q, col + 64, cols, code + 2);
+                if (lane == 0) a.scale[(size_t)kb * a.lds + r] = scale;
             }
         }
     }
@@ -331,12 +359,8 @@ __global__ __launch_bounds__(kThreads) void fp8_quant_weight_kernel(const T* __r
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
         const int r = p * 16 + row;
-        load8<T, VEC>(src + (size_t)(r < rows ? r : 0) * k, r < rows ? col : 0, r < rows ? k : 0, v[p]);
+        m = max_nan(m, load8<T, VEC>(src + (size_t)(r < rows ? r : 0) * k, r < rows ? col : 0, r < rows ? k : 0, v[p]));
     }
-#pragma unroll
-    for (int p = 0; p < 8; ++p)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[p][j]));
 #pragma unroll
     for (int d = 16; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
@@ -349,36 +373,41 @@ __global__ __launch_bounds__(kThreads) void fp8_quant_weight_kernel(const T* __r
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
         const int r = p * 16 + row;
-        if (r < rows) store_codes(dst + (size_t)r * ldq, col, k, codes8(v[p], b));
+        uint32_t code[2];
+        codes_of<8>(v[p], b, code);
+        if (r < rows) store_codes(dst + (size_t)r * ldq, col, k, code);
     }
 }
 
 template <typename T>
 bool rows_aligned(const void* p, size_t ld) { return ((uintptr_t)p & 15u) == 0 && ld * sizeof(T) % 16 == 0; }
 
-template <typename T>
-int quant_t(const Fp8QuantArgs& a, cudaStream_t stream) {
+template <typename T, bool VEC>
+int quant_v(const Fp8QuantArgs& a, cudaStream_t stream) {
     const int kb = (a.cols + 127) / 128;
     const size_t blocks = (size_t)a.rows * kb;
-    // small calls: one block per half-warp, so that every SM has some
-    const int share = blocks >= (size_t)148 * 4 * kShare ? kShare : kUnits;
+    // four blocks per group of lanes; small calls one, so that every SM has some
+    const int share = blocks >= (size_t)148 * 8 * kUnits ? 4 * kUnits : kUnits;
     const size_t grid = (blocks + share - 1) / share;
     if (grid > 0x7fffffffu) return XMOE_ERR_LIMIT;
-    if (rows_aligned<T>(a.x, a.ldx)) fp8_quant_kernel<T, true><<<(unsigned)grid, kThreads, 0, stream>>>(a, kb, share);
-    else fp8_quant_kernel<T, false><<<(unsigned)grid, kThreads, 0, stream>>>(a, kb, share);
+    if (a.topk_row) fp8_quant_kernel<T, VEC, true><<<(unsigned)grid, kThreads, 0, stream>>>(a, kb, share);
+    else fp8_quant_kernel<T, VEC, false><<<(unsigned)grid, kThreads, 0, stream>>>(a, kb, share);
     return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
+}
+template <typename T>
+int quant_t(const Fp8QuantArgs& a, cudaStream_t stream) {
+    return rows_aligned<T>(a.x, a.ldx) ? quant_v<T, true>(a, stream) : quant_v<T, false>(a, stream);
 }
 
 template <typename T, int ACT, bool BACKWARD>
 int glu_act(const Fp8QuantArgs& a, cudaStream_t stream) {
     const int kb = (a.cols + 127) / 128;
-    const int tile_rows = kb >= 4 ? 4 : 16;
-    const int tiles = (a.rows + tile_rows - 1) / tile_rows;
-    const dim3 grid(tiles < 148 * 8 ? tiles : 148 * 8);
+    const size_t ctas = ((size_t)a.rows * kb + kUnits - 1) / kUnits, most = 148 * (BACKWARD ? 5 : 4);
+    const unsigned grid = (unsigned)(ctas < most ? ctas : most);
     const bool vec = rows_aligned<T>(a.x, a.ldx) && a.cols * sizeof(T) % 16 == 0 &&
                      (!BACKWARD || (((uintptr_t)a.da | (uintptr_t)a.dh) & 15u) == 0);
-    if (vec) glu_kernel<T, true, ACT, BACKWARD><<<grid, kThreads, 0, stream>>>(a, kb, tile_rows);
-    else glu_kernel<T, false, ACT, BACKWARD><<<grid, kThreads, 0, stream>>>(a, kb, tile_rows);
+    if (vec) glu_kernel<T, true, ACT, BACKWARD><<<grid, kThreads, 0, stream>>>(a, kb);
+    else glu_kernel<T, false, ACT, BACKWARD><<<grid, kThreads, 0, stream>>>(a, kb);
     return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
 }
 template <typename T, bool BACKWARD>
