@@ -81,8 +81,8 @@ int make_tmap_codes(CUtensorMap* out, const void* base, uint64_t inner, uint64_t
     cuuint32_t box[3] = {128, box_rows, 1};
     cuuint32_t estr[3] = {1, 1, 1};
     const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, mats ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? XMOE_OK : XMOE_ERR_CUDA;
 }
 

@@ -53,9 +53,9 @@ __device__ __forceinline__ void mma_fp8(uint32_t d_tmem, uint32_t a_lo, uint32_t
 __host__ __device__ constexpr uint32_t idesc_fp8(uint32_t m, uint32_t n, bool a_trans, bool b_trans) {
     return (1u << 4) | ((a_trans ? 1u : 0u) << 15) | ((b_trans ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
-// A transposed operand (features contiguous): a K step of 32 is 32 rows of 128 bytes; both stride fields are the 1024
-// bytes between 8-row groups (the tile is one swizzle atom wide, so only one of them is used).
-__device__ __forceinline__ uint32_t desc_lo_trans(uint32_t smem_addr) { return ((smem_addr & 0x3ffffu) >> 4) | ((1024u >> 4) << 16); }
+// A transposed operand (features contiguous): a K step of 32 is 32 rows of 128 bytes, 1024 bytes between 8-row groups, one
+// box (16 KB) between swizzle atoms of 128 features.
+__device__ __forceinline__ uint32_t desc_lo_trans(uint32_t smem_addr) { return ((smem_addr & 0x3ffffu) >> 4) | (((uint32_t)kBoxBytes >> 4) << 16); }
 constexpr uint32_t kTransStep = (32u * 128u) >> 4;
 // a * b + c on two fp32 at once
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -356,7 +356,8 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
 // Each CTA of the pair stages its 128 tokens and 128 of the 256 features: 32 KB per 128 columns of K instead of 48.
 constexpr int kPairStages = 6, kPairThreads = 384, kPairEpiWarps = 8;
 constexpr int kPairStageBytes = 2 * kBoxBytes;
-constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStageBytes + 1024 + (size_t)(3 * kMaxMats + 4) * 4;
+constexpr int kPairSlots = kPairStages + 2;  // of token scales: as in Cfg, with two accumulators
+constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStageBytes + kPairSlots * 512 + 1024 + (size_t)(3 * kMaxMats + 4) * 4;
 static_assert(kPairSmem <= 232448, "shared memory");
 // 128 sums and two 32-column reads per epilogue thread: these warps take registers over from the single-purpose ones. 384
 // threads are launched with 168 each; 128 * 40 + 256 * 232 = 384 * 168.
@@ -373,9 +374,11 @@ template <bool TRANS, typename OT>
 __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __grid_constant__ Fp8GemmArgs a) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + (size_t)kPairStages * kPairStageBytes);
+    float* scales = reinterpret_cast<float*>(smem + (size_t)kPairStages * kPairStageBytes);  // [kPairSlots][128] this CTA's tokens'
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(scales + kPairSlots * 128);
     uint64_t* empty_bar = full_bar + 8;
-    uint64_t* acc_full = empty_bar + 8;  // [2] in each CTA
+    uint64_t* sc_full = empty_bar + 8;
+    uint64_t* acc_full = sc_full + 8;    // [2] in each CTA
     uint64_t* acc_empty = acc_full + 2;  // [2] leader: both CTAs' epilogue warps
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile uint32_t* abort_flag = tmem_slot + 1;
@@ -393,6 +396,7 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
             mbar_init(&full_bar[s], rank == 0 ? 2 : 1);  // leader: + the peer's report that its stage landed
             mbar_init(&empty_bar[s], 1);
         }
+        for (int s = 0; s < kPairSlots; ++s) mbar_init(&sc_full[s], 1);
         for (int s = 0; s < 2; ++s) {
             mbar_init(&acc_full[s], 1);
             mbar_init(&acc_empty[s], 2 * kPairEpiWarps);
@@ -421,11 +425,15 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
         if (warp == 0 && lane == 0) {
-            uint32_t s = 0, ph = 0;
+            uint32_t s = 0, ph = 0, slot = 0;
             bool ok = true;
             for (int item = first; item < total_tiles && ok; item += stride) {
                 const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, 256);
                 const int f0 = t.wt * 256 + rank * 128, row = t.row0 + rank * 128;
+                // scales of this CTA's tokens: a multiple of 16 bytes inside the block's row; none past the last row
+                const int sc_rows = min(128, ((a.rows + 3) & ~3) - row);
+                const uint32_t sc_bytes = sc_rows > 0 ? (uint32_t)sc_rows * 4u : 0u;
+                const float* sc = a.x_scale + row;
                 for (int kb = 0; kb < kb_total; ++kb) {
                     if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_MMA)) {
                         ok = false;
@@ -436,7 +444,10 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
                     tma_load_2d(st, &a.tm_x, kb * 128, row, &full_bar[s]);
                     if (TRANS) tma_load_3d(st + kBoxBytes, &a.tm_w, f0, kb * 128, t.e, &full_bar[s]);
                     else tma_load_3d(st + kBoxBytes, &a.tm_w, kb * 128, f0, t.e, &full_bar[s]);
+                    mbar_expect_tx(&sc_full[slot], sc_bytes);
+                    if (sc_bytes) tma_load_1d(scales + slot * 128, sc + (size_t)kb * a.lds, sc_bytes, &sc_full[slot]);
                     if (++s == (uint32_t)kPairStages) { s = 0; ph ^= 1u; }
+                    if (++slot == (uint32_t)kPairSlots) slot = 0;
                 }
             }
         } else if (warp == 1 && lane == 0 && rank == 0) {
@@ -486,7 +497,8 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
         const int q = warp & 3, part = (warp - 4) >> 2;
         const uint32_t src0 = tmem_base + ((uint32_t)(q * 32) << 16) + part * 128;
         const uint32_t leader_empty = map_to_cta(smem_u32(acc_empty), 0);
-        uint32_t acc = 0, acc_ph = 0;
+        uint32_t acc = 0, acc_ph = 0, slot = 0, slot_ph = 0;
+        const size_t ws_step = TRANS ? w_blocks : 1;
         bool ok = true;
         for (int item = first; item < total_tiles && ok; item += stride) {
             const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, 256);
@@ -494,59 +506,44 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
             const bool live = m < t.count - t.nt_idx * 256;
             const int fb = min(t.wt * 2 + part, w_blocks - 1);  // a block past the end: its values are not stored
             const float* ws = a.w_scale + (size_t)t.e * w_blocks * kb_total + (TRANS ? (size_t)fb : (size_t)fb * kb_total);
-            const size_t ws_step = TRANS ? w_blocks : 1;
-            const float* xs = a.x_scale + (live ? t.row0 + m : 0);
-            // scales of the next two blocks are in flight
-            float x_next[2], w_next[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int kb = min(i, kb_total - 1);
-                x_next[i] = xs[(size_t)kb * a.lds];
-                w_next[i] = ws[kb * ws_step];
-            }
             float2 sum[64];
 #pragma unroll
             for (int j = 0; j < 64; ++j) sum[j] = make_float2(0.f, 0.f);
-            bool ready = false;
-            for (int kb0 = 0; kb0 < kb_total && ok; kb0 += 2) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (kb0 + i >= kb_total) break;
-                    if (!ready && !mbar_wait(&acc_full[acc], acc_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_ACC)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t src = src0 + acc * 256;
-                    uint32_t v0[32], v1[32];
-                    tmem_ld32(src, v0);
-                    const float s = x_next[i] * w_next[i];
-                    const float2 s2 = make_float2(s, s);
-                    {
-                        const int kb = min(kb0 + i + 2, kb_total - 1);
-                        x_next[i] = xs[(size_t)kb * a.lds];
-                        w_next[i] = ws[kb * ws_step];
-                    }
-                    tmem_wait_for<32>(v0);
-                    tmem_ld32(src + 32, v1);
-                    add_scaled32(sum, v0, s2);
-                    tmem_wait_for<32>(v1);
-                    tmem_ld32(src + 64, v0);
-                    add_scaled32(sum + 16, v1, s2);
-                    tmem_wait_for<32>(v0);
-                    tmem_ld32(src + 96, v1);
-                    add_scaled32(sum + 32, v0, s2);
-                    tmem_wait_for<32>(v1);
-                    // everything is in registers: hand the accumulator back, and look whether the next one is there
-                    // while the last columns are added
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(leader_empty + acc * 8u);
-                    acc ^= 1u;
-                    acc_ph ^= acc ^ 1u;
-                    ready = mbar_test_wait(&acc_full[acc], acc_ph);
-                    add_scaled32(sum + 48, v1, s2);
+            float ws_lane = 0.f;  // the weight's scales of 32 blocks, one per lane: no global load inside the loop
+            for (int kb = 0; kb < kb_total; ++kb) {
+                if ((kb & 31) == 0) ws_lane = kb + lane < kb_total ? ws[(size_t)(kb + lane) * ws_step] : 0.f;
+                if (!mbar_wait(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
+                    ok = false;
+                    break;
                 }
+                const float s = scales[slot * 128 + q * 32 + lane] * __shfl_sync(0xffffffffu, ws_lane, kb & 31);
+                const float2 s2 = make_float2(s, s);
+                if (!mbar_wait(&acc_full[acc], acc_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_ACC)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t src = src0 + acc * 256;
+                uint32_t v0[32], v1[32];
+                tmem_ld32(src, v0);
+                tmem_wait_for<32>(v0);
+                tmem_ld32(src + 32, v1);
+                add_scaled32(sum, v0, s2);
+                tmem_wait_for<32>(v1);
+                tmem_ld32(src + 64, v0);
+                add_scaled32(sum + 16, v1, s2);
+                tmem_wait_for<32>(v0);
+                tmem_ld32(src + 96, v1);
+                add_scaled32(sum + 32, v0, s2);
+                tmem_wait_for<32>(v1);
+                // everything is in registers: hand the accumulator back before the last columns are added
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(leader_empty + acc * 8u);
+                acc ^= 1u;
+                acc_ph ^= acc ^ 1u;
+                if (++slot == (uint32_t)kPairSlots) { slot = 0; slot_ph ^= 1u; }
+                add_scaled32(sum + 48, v1, s2);
             }
             if (!ok) break;
             const int f = t.wt * 256 + part * 128;
