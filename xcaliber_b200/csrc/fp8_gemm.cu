@@ -357,7 +357,10 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
 constexpr int kPairStages = 6, kPairThreads = 384, kPairEpiWarps = 8;
 constexpr int kPairStageBytes = 2 * kBoxBytes;
 constexpr int kPairSlots = kPairStages + 2;  // of token scales: as in Cfg, with two accumulators
-constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStageBytes + kPairSlots * 512 + 1024 + (size_t)(3 * kMaxMats + 4) * 4;
+// Output goes out by way of shared memory, 64 bytes of 32 rows per warp at a time: a store instruction then writes eight
+// rows' 64 bytes instead of 16 bytes of 32 rows, of which the load / store unit takes one line per cycle.
+constexpr int kOutBytes = 32 * 64;
+constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStageBytes + kPairSlots * 512 + kPairEpiWarps * kOutBytes + 1024 + (size_t)(3 * kMaxMats + 4) * 4;
 static_assert(kPairSmem <= 232448, "shared memory");
 // 128 sums and two 32-column reads per epilogue thread: these warps take registers over from the single-purpose ones. 384
 // threads are launched with 168 each; 128 * 40 + 256 * 232 = 384 * 168.
@@ -375,7 +378,8 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     float* scales = reinterpret_cast<float*>(smem + (size_t)kPairStages * kPairStageBytes);  // [kPairSlots][128] this CTA's tokens'
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(scales + kPairSlots * 128);
+    uint8_t* out_tiles = reinterpret_cast<uint8_t*>(scales + kPairSlots * 128);
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(out_tiles + kPairEpiWarps * kOutBytes);
     uint64_t* empty_bar = full_bar + 8;
     uint64_t* sc_full = empty_bar + 8;
     uint64_t* acc_full = sc_full + 8;    // [2] in each CTA
@@ -547,21 +551,38 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
             }
             if (!ok) break;
             const int f = t.wt * 256 + part * 128;
-            if (live && f < a.out_features) {
-                OT* dst = reinterpret_cast<OT*>(a.out) + (size_t)(t.row0 + m) * a.ldo + f;
-                constexpr int kVec = 16 / sizeof(OT);
+            const int rows = min(32, t.count - t.nt_idx * 256 - (m - lane));  // this warp's live rows (may be <= 0)
+            if (rows > 0 && f < a.out_features) {
+                OT* dst = reinterpret_cast<OT*>(a.out) + (size_t)(t.row0 + m - lane) * a.ldo + f;
                 if (a.out_vec && f + 128 <= a.out_features) {
+                    constexpr int kVec = 16 / sizeof(OT), kChunk = 4 * kVec;
+                    // 16-byte piece p of row r sits at piece p ^ (r / 2) & 3: neither side meets a bank conflict
+                    uint8_t* tile = out_tiles + (warp - 4) * kOutBytes;
 #pragma unroll
-                    for (int j = 0; j < 128; j += kVec) {
-                        Pack<OT, kVec> o;
+                    for (int c = 0; c < 128; c += kChunk) {
 #pragma unroll
-                        for (int i = 0; i < kVec; ++i) o.v[i] = from_f32<OT>((j + i) & 1 ? sum[(j + i) / 2].y : sum[(j + i) / 2].x);
-                        store_pack<OT, kVec>(dst + j, o);
+                        for (int p = 0; p < 4; ++p) {
+                            Pack<OT, kVec> o;
+#pragma unroll
+                            for (int i = 0; i < kVec; ++i) {
+                                const int j = c + p * kVec + i;
+                                o.v[i] = from_f32<OT>(j & 1 ? sum[j / 2].y : sum[j / 2].x);
+                            }
+                            *reinterpret_cast<uint4*>(tile + lane * 64 + ((p ^ (lane >> 1)) & 3) * 16) = *reinterpret_cast<const uint4*>(&o);
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int r = i * 8 + (lane >> 2), p = lane & 3;
+                            const uint4 o = *reinterpret_cast<const uint4*>(tile + r * 64 + ((p ^ (r >> 1)) & 3) * 16);
+                            if (r < rows) *reinterpret_cast<uint4*>(dst + (size_t)r * a.ldo + c + p * kVec) = o;
+                        }
+                        __syncwarp();
                     }
-                } else {
+                } else if (live) {
 #pragma unroll
                     for (int j = 0; j < 128; ++j)
-                        if (f + j < a.out_features) dst[j] = from_f32<OT>(j & 1 ? sum[j / 2].y : sum[j / 2].x);
+                        if (f + j < a.out_features) dst[(size_t)lane * a.ldo + j] = from_f32<OT>(j & 1 ? sum[j / 2].y : sum[j / 2].x);
                 }
             }
         }
