@@ -86,6 +86,21 @@ int make_tmap_codes(CUtensorMap* out, const void* base, uint64_t inner, uint64_t
     return r == CUDA_SUCCESS ? XMOE_OK : XMOE_ERR_CUDA;
 }
 
+// Block-major token scales: fp32 [blocks][rows], rows of a block `ld` floats apart, boxes of box_blocks x box_rows.
+int make_tmap_scales(CUtensorMap* out, const float* base, uint64_t rows, uint64_t blocks, uint64_t ld, uint32_t box_rows,
+                     uint32_t box_blocks) {
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn) return XMOE_ERR_CUDA;
+    cuuint64_t dims[2] = {rows, blocks};
+    cuuint64_t strides[1] = {ld * 4};
+    cuuint32_t box[2] = {box_rows, box_blocks};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? XMOE_OK : XMOE_ERR_CUDA;
+}
+
 int num_sms() {  // of the current device
     static int n_dev[kMaxDevices] = {};
     const int dev = device_slot();
@@ -667,13 +682,16 @@ int run_fp8_gemm(const void* x, int ldx, const float* x_scale, int lds, const vo
     if (rc) return rc;
     rc = make_tmap_codes(&a.tm_x, x, (uint64_t)contraction, (uint64_t)rows, 0, (uint64_t)ldx, 0, (uint32_t)(tile == 256 ? 128 : tile));
     if (rc) return rc;
-    a.x_scale = x_scale;
+    // lds >= rows rounded up to 4, so the view may end there
+    const int tile_rows = tile == 256 ? 128 : tile;
+    rc = make_tmap_scales(&a.tm_s, x_scale, ((uint64_t)rows + 3) / 4 * 4, ((uint64_t)contraction + 127) / 128, (uint64_t)lds,
+                          (uint32_t)tile_rows, tile == 256 ? 2 : 4);
+    if (rc) return rc;
     a.w_scale = w_scale;
     a.counts = counts;
     a.offsets = offsets;
     a.out = out;
     a.rows = rows;
-    a.lds = lds;
     a.ldo = ldo;
     a.mats = mats;
     a.out_features = features;

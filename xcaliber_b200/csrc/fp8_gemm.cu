@@ -82,10 +82,9 @@ struct Cfg {
     static constexpr int kTmemCols = kAcc * TN;
     static constexpr int kStageBytes = kBoxBytes + TN * 128;
     static constexpr int kStages = TN >= 128 ? 6 : (TN >= 64 ? 8 : 10);
-    // a scale slot is written again kStages + kAcc blocks later: by then the MMA of the block that used the stage kStages
-    // blocks ago has been issued, so the epilogue has drained the block kAcc before that one
-    static constexpr int kSlots = kStages + kAcc;
-    static constexpr size_t kTail = (size_t)kSlots * TN * 4 + 1024;
+    static constexpr int kGroup = 4, kSlots = 4;                  // blocks whose token scales come together; such groups in flight
+    static_assert(kStages % 2 == 0 && kAcc % 2 == 0, "two issuing threads take the blocks in turn");
+    static constexpr size_t kTail = (size_t)kSlots * kGroup * TN * 4 + 1024;
     static constexpr size_t kSmem = 1024 + (size_t)kStages * kStageBytes + kTail + (size_t)(3 * kMaxMats + 4) * 4;
     static_assert(kSmem <= 232448, "shared memory");
     static_assert(kTmemCols >= 32 && kTmemCols <= 512, "tensor memory");
@@ -133,11 +132,12 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
     using C = Cfg<TN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    float* scales = reinterpret_cast<float*>(smem + (size_t)C::kStages * C::kStageBytes);  // [kSlots][TN] the block's token scales
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(scales + C::kSlots * TN);
+    float* scales = reinterpret_cast<float*>(smem + (size_t)C::kStages * C::kStageBytes);  // [kSlots][kGroup][TN] the tokens'
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(scales + C::kSlots * C::kGroup * TN);
     uint64_t* empty_bar = full_bar + 16;
     uint64_t* sc_full = empty_bar + 16;  // [kSlots]
-    uint64_t* acc_full = sc_full + 16;
+    uint64_t* sc_empty = sc_full + 4;
+    uint64_t* acc_full = sc_empty + 4;
     uint64_t* acc_empty = acc_full + 4;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 4);
     volatile uint32_t* abort_flag = tmem_slot + 1;
@@ -154,7 +154,10 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
             mbar_init(&full_bar[s], 1);
             mbar_init(&empty_bar[s], 1);
         }
-        for (int s = 0; s < C::kSlots; ++s) mbar_init(&sc_full[s], 1);
+        for (int s = 0; s < C::kSlots; ++s) {
+            mbar_init(&sc_full[s], 1);
+            mbar_init(&sc_empty[s], C::kEpiWarps);
+        }
         for (int s = 0; s < C::kAcc; ++s) {
             mbar_init(&acc_full[s], 1);
             mbar_init(&acc_empty[s], C::kEpiWarps);
@@ -163,6 +166,7 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
         mbar_fence_init();
         prefetch_tmap(&a.tm_w);
         prefetch_tmap(&a.tm_x);
+        prefetch_tmap(&a.tm_s);
     }
     if (warp == 1) {
         tmem_alloc(tmem_slot, C::kTmemCols);
@@ -186,33 +190,38 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
     if (warp < 4) {
         if (warp == 0) {
             if (lane == 0) {
-                uint32_t s = 0, ph = 0, slot = 0;
+                uint32_t s = 0, ph = 0, slot = 0, slot_ph = 0;
                 bool ok = true;
                 for (int item = first; item < total_tiles && ok; item += stride) {
                     const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, TN);
-                    // scales of this tile's tokens: a multiple of 16 bytes, inside the block's row (lds >= rows, both ends
-                    // multiples of 4)
-                    const uint32_t sc_bytes = (uint32_t)min(TN, ((a.rows + 3) & ~3) - t.row0) * 4u;
-                    const float* sc = a.x_scale + t.row0;
                     for (int kb = kb_lo; kb < kb_hi; ++kb) {
                         if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_MMA)) {
                             ok = false;
                             break;
+                        }
+                        if ((kb - kb_lo) % C::kGroup == 0) {
+                            if (!mbar_wait(&sc_empty[slot], slot_ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_EPI)) {
+                                ok = false;
+                                break;
+                            }
+                            mbar_expect_tx(&sc_full[slot], C::kGroup * TN * 4);
+                            tma_load_2d(scales + slot * C::kGroup * TN, &a.tm_s, t.row0, kb, &sc_full[slot]);
+                            if (++slot == (uint32_t)C::kSlots) { slot = 0; slot_ph ^= 1u; }
                         }
                         uint8_t* st = smem + (size_t)s * C::kStageBytes;
                         mbar_expect_tx(&full_bar[s], C::kStageBytes);
                         if (TRANS) tma_load_3d(st, &a.tm_w, t.wt * 128, kb * 128, t.e, &full_bar[s]);
                         else tma_load_3d(st, &a.tm_w, kb * 128, t.wt * 128, t.e, &full_bar[s]);
                         tma_load_2d(st + kBoxBytes, &a.tm_x, kb * 128, t.row0, &full_bar[s]);
-                        mbar_expect_tx(&sc_full[slot], sc_bytes);
-                        tma_load_1d(scales + slot * TN, sc + (size_t)kb * a.lds, sc_bytes, &sc_full[slot]);
                         if (++s == (uint32_t)C::kStages) { s = 0; ph ^= 1u; }
-                        if (++slot == (uint32_t)C::kSlots) slot = 0;
                     }
                 }
             }
-        } else if (warp == 1) {
+        } else if (warp == 1 || warp == 3) {
+            // two issuing threads take the blocks in turn: one alone spends ~375 cycles on a block's six tcgen05 instructions
+            // and as long on its waits
             if (lane == 0) {
+                const uint32_t mine = warp == 1 ? 0u : 1u;
                 constexpr uint32_t kStage16 = C::kStageBytes >> 4;
                 const uint32_t w_lo0 = TRANS ? desc_lo_trans(smem_u32(smem)) : umma_desc_lo_sw128(smem_u32(smem));
                 const uint32_t x_lo0 = umma_desc_lo_sw128(smem_u32(smem + kBoxBytes));
@@ -224,18 +233,20 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
                     const int n_tok = min(TN, t.count - t.nt_idx * TN);
                     const uint32_t idesc = idesc_fp8(128, (uint32_t)((n_tok + 15) & ~15), TRANS, false);
                     for (int kb = kb_lo; kb < kb_hi; ++kb) {
-                        if (!mbar_wait(&acc_empty[acc], acc_ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_EPI) ||
-                            !mbar_wait(&full_bar[s], ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        const uint32_t w_lo = w_lo0 + s * kStage16, x_lo = x_lo0 + s * kStage16;
+                        if ((s & 1u) == mine) {
+                            if (!mbar_wait(&acc_empty[acc], acc_ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_EPI) ||
+                                !mbar_wait(&full_bar[s], ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            const uint32_t w_lo = w_lo0 + s * kStage16, x_lo = x_lo0 + s * kStage16;
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            mma_fp8<false>(tmem_base + acc * TN, w_lo + kk * kWStep, x_lo + kk * 2, idesc, kk ? 1u : 0u);
-                        tc_commit(&empty_bar[s]);
-                        tc_commit(&acc_full[acc]);
+                            for (int kk = 0; kk < 4; ++kk)
+                                mma_fp8<false>(tmem_base + acc * TN, w_lo + kk * kWStep, x_lo + kk * 2, idesc, kk ? 1u : 0u);
+                            tc_commit(&empty_bar[s]);
+                            tc_commit(&acc_full[acc]);
+                        }
                         if (++s == (uint32_t)C::kStages) { s = 0; ph ^= 1u; }
                         if (++acc == (uint32_t)C::kAcc) { acc = 0; acc_ph ^= 1u; }
                     }
@@ -264,13 +275,14 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
             for (int kb = kb_lo; kb < kb_hi; ++kb) {
                 if (((kb - kb_lo) & 31) == 0) ws_lane = kb + lane < kb_hi ? ws[(size_t)(kb + lane) * (TRANS ? w_tiles : 1)] : 0.f;
                 const float sw = __shfl_sync(0xffffffffu, ws_lane, (kb - kb_lo) & 31);
-                if (!mbar_wait(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA) ||
+                const int g = (kb - kb_lo) % C::kGroup;
+                if ((g == 0 && !mbar_wait(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) ||
                     !mbar_wait(&acc_full[acc], acc_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_ACC)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const float4* xs = reinterpret_cast<const float4*>(scales + slot * TN + col0);
+                const float4* xs = reinterpret_cast<const float4*>(scales + (slot * C::kGroup + g) * TN + col0);
                 const uint32_t src = lane_addr + acc * TN;
                 constexpr int kN = C::kCols / C::kChunk;
                 if (n_tok > C::kCols - C::kChunk) {  // all chunks hold tokens: the next read is in flight while one is added
@@ -297,7 +309,10 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&acc_empty[acc]);
                 if (++acc == (uint32_t)C::kAcc) { acc = 0; acc_ph ^= 1u; }
-                if (++slot == (uint32_t)C::kSlots) { slot = 0; slot_ph ^= 1u; }
+                if (g == C::kGroup - 1 || kb + 1 == kb_hi) {  // done with the group's scales
+                    if (lane == 0) mbar_arrive(&sc_empty[slot]);
+                    if (++slot == (uint32_t)C::kSlots) { slot = 0; slot_ph ^= 1u; }
+                }
             }
             if (split > 1) {
                 // Partial sums to the CTA that stores the column: rank r stores columns [r * TN / split, ..). Once every
@@ -356,11 +371,11 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
 // Each CTA of the pair stages its 128 tokens and 128 of the 256 features: 32 KB per 128 columns of K instead of 48.
 constexpr int kPairStages = 6, kPairThreads = 384, kPairEpiWarps = 8;
 constexpr int kPairStageBytes = 2 * kBoxBytes;
-constexpr int kPairSlots = kPairStages + 2;  // of token scales: as in Cfg, with two accumulators
+constexpr int kPairGroup = 2, kPairSlots = 4;  // token scales: as in Cfg
 // Output goes out by way of shared memory, 64 bytes of 32 rows per warp at a time: a store instruction then writes eight
 // rows' 64 bytes instead of 16 bytes of 32 rows, of which the load / store unit takes one line per cycle.
 constexpr int kOutBytes = 32 * 64;
-constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStageBytes + kPairSlots * 512 + kPairEpiWarps * kOutBytes + 1024 + (size_t)(3 * kMaxMats + 4) * 4;
+constexpr size_t kPairSmem = 1024 + (size_t)kPairStages * kPairStageBytes + kPairSlots * kPairGroup * 512 + kPairEpiWarps * kOutBytes + 512 + (size_t)(3 * kMaxMats + 4) * 4;
 static_assert(kPairSmem <= 232448, "shared memory");
 // 128 sums and two 32-column reads per epilogue thread: these warps take registers over from the single-purpose ones. 384
 // threads are launched with 168 each; 128 * 40 + 256 * 232 = 384 * 168.
@@ -377,16 +392,17 @@ template <bool TRANS, typename OT>
 __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __grid_constant__ Fp8GemmArgs a) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    float* scales = reinterpret_cast<float*>(smem + (size_t)kPairStages * kPairStageBytes);  // [kPairSlots][128] this CTA's tokens'
-    uint8_t* out_tiles = reinterpret_cast<uint8_t*>(scales + kPairSlots * 128);
+    float* scales = reinterpret_cast<float*>(smem + (size_t)kPairStages * kPairStageBytes);  // [kPairSlots][kPairGroup][128] this CTA's tokens'
+    uint8_t* out_tiles = reinterpret_cast<uint8_t*>(scales + kPairSlots * kPairGroup * 128);
     uint64_t* full_bar = reinterpret_cast<uint64_t*>(out_tiles + kPairEpiWarps * kOutBytes);
     uint64_t* empty_bar = full_bar + 8;
     uint64_t* sc_full = empty_bar + 8;
-    uint64_t* acc_full = sc_full + 8;    // [2] in each CTA
+    uint64_t* sc_empty = sc_full + 4;
+    uint64_t* acc_full = sc_empty + 4;   // [2] in each CTA
     uint64_t* acc_empty = acc_full + 2;  // [2] leader: both CTAs' epilogue warps
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile uint32_t* abort_flag = tmem_slot + 1;
-    int* counts = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full_bar) + 1024);
+    int* counts = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(full_bar) + 512);
     int* offsets = counts + kMaxMats;
     int* prefix = offsets + kMaxMats;
 
@@ -400,7 +416,10 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
             mbar_init(&full_bar[s], rank == 0 ? 2 : 1);  // leader: + the peer's report that its stage landed
             mbar_init(&empty_bar[s], 1);
         }
-        for (int s = 0; s < kPairSlots; ++s) mbar_init(&sc_full[s], 1);
+        for (int s = 0; s < kPairSlots; ++s) {
+            mbar_init(&sc_full[s], 1);
+            mbar_init(&sc_empty[s], kPairEpiWarps);
+        }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&acc_full[s], 1);
             mbar_init(&acc_empty[s], 2 * kPairEpiWarps);
@@ -409,6 +428,7 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
         mbar_fence_init();
         prefetch_tmap(&a.tm_w);
         prefetch_tmap(&a.tm_x);
+        prefetch_tmap(&a.tm_s);
     }
     if (warp == 1) {
         tmem_alloc_pair(tmem_slot, 512);
@@ -429,32 +449,35 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
         if (warp == 0 && lane == 0) {
-            uint32_t s = 0, ph = 0, slot = 0;
+            uint32_t s = 0, ph = 0, slot = 0, slot_ph = 0;
             bool ok = true;
             for (int item = first; item < total_tiles && ok; item += stride) {
                 const TileInfo t = tile_decode(item, prefix, counts, offsets, a.mats, 256);
                 const int f0 = t.wt * 256 + rank * 128, row = t.row0 + rank * 128;
-                // scales of this CTA's tokens: a multiple of 16 bytes inside the block's row; none past the last row
-                const int sc_rows = min(128, ((a.rows + 3) & ~3) - row);
-                const uint32_t sc_bytes = sc_rows > 0 ? (uint32_t)sc_rows * 4u : 0u;
-                const float* sc = a.x_scale + row;
                 for (int kb = 0; kb < kb_total; ++kb) {
                     if (!mbar_wait(&empty_bar[s], ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_MMA)) {
                         ok = false;
                         break;
+                    }
+                    if (kb % kPairGroup == 0) {
+                        if (!mbar_wait(&sc_empty[slot], slot_ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_EPI)) {
+                            ok = false;
+                            break;
+                        }
+                        mbar_expect_tx(&sc_full[slot], kPairGroup * 512);
+                        tma_load_2d(scales + slot * kPairGroup * 128, &a.tm_s, row, kb, &sc_full[slot]);
+                        if (++slot == (uint32_t)kPairSlots) { slot = 0; slot_ph ^= 1u; }
                     }
                     uint8_t* st = smem + (size_t)s * kPairStageBytes;
                     mbar_expect_tx(&full_bar[s], kPairStageBytes);
                     tma_load_2d(st, &a.tm_x, kb * 128, row, &full_bar[s]);
                     if (TRANS) tma_load_3d(st + kBoxBytes, &a.tm_w, f0, kb * 128, t.e, &full_bar[s]);
                     else tma_load_3d(st + kBoxBytes, &a.tm_w, kb * 128, f0, t.e, &full_bar[s]);
-                    mbar_expect_tx(&sc_full[slot], sc_bytes);
-                    if (sc_bytes) tma_load_1d(scales + slot * 128, sc + (size_t)kb * a.lds, sc_bytes, &sc_full[slot]);
                     if (++s == (uint32_t)kPairStages) { s = 0; ph ^= 1u; }
-                    if (++slot == (uint32_t)kPairSlots) slot = 0;
                 }
             }
-        } else if (warp == 1 && lane == 0 && rank == 0) {
+        } else if ((warp == 1 || warp == 3) && lane == 0 && rank == 0) {
+            const uint32_t mine = warp == 1 ? 0u : 1u;  // two issuing threads take the blocks, and so the accumulators, in turn
             constexpr uint32_t kStage16 = kPairStageBytes >> 4;
             constexpr uint32_t idesc = idesc_fp8(256, 256, false, TRANS);
             constexpr uint32_t kWStep = TRANS ? kTransStep : 2u;
@@ -464,18 +487,20 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
             bool ok = true;
             for (int item = first; item < total_tiles && ok; item += stride) {
                 for (int kb = 0; kb < kb_total; ++kb) {
-                    if (!mbar_wait(&acc_empty[acc], acc_ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_EPI) ||
-                        !mbar_wait(&full_bar[s], ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t w_lo = w_lo0 + s * kStage16, x_lo = x_lo0 + s * kStage16;
+                    if (acc == mine) {
+                        if (!mbar_wait(&acc_empty[acc], acc_ph ^ 1u, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_EPI) ||
+                            !mbar_wait(&full_bar[s], ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t w_lo = w_lo0 + s * kStage16, x_lo = x_lo0 + s * kStage16;
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        mma_fp8<true>(tmem_base + acc * 256, x_lo + kk * 2, w_lo + kk * kWStep, idesc, kk ? 1u : 0u);
-                    tc_commit_pair_mask(smem_u32(&empty_bar[s]), 3);
-                    tc_commit_pair_mask(smem_u32(&acc_full[acc]), 3);
+                        for (int kk = 0; kk < 4; ++kk)
+                            mma_fp8<true>(tmem_base + acc * 256, x_lo + kk * 2, w_lo + kk * kWStep, idesc, kk ? 1u : 0u);
+                        tc_commit_pair_mask(smem_u32(&empty_bar[s]), 3);
+                        tc_commit_pair_mask(smem_u32(&acc_full[acc]), 3);
+                    }
                     if (++s == (uint32_t)kPairStages) { s = 0; ph ^= 1u; }
                     acc ^= 1u;
                     acc_ph ^= acc ^ 1u;
@@ -516,11 +541,12 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
             float ws_lane = 0.f;  // the weight's scales of 32 blocks, one per lane: no global load inside the loop
             for (int kb = 0; kb < kb_total; ++kb) {
                 if ((kb & 31) == 0) ws_lane = kb + lane < kb_total ? ws[(size_t)(kb + lane) * ws_step] : 0.f;
-                if (!mbar_wait(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
+                const int g = kb % kPairGroup;
+                if (g == 0 && !mbar_wait(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
                     ok = false;
                     break;
                 }
-                const float s = scales[slot * 128 + q * 32 + lane] * __shfl_sync(0xffffffffu, ws_lane, kb & 31);
+                const float s = scales[(slot * kPairGroup + g) * 128 + q * 32 + lane] * __shfl_sync(0xffffffffu, ws_lane, kb & 31);
                 const float2 s2 = make_float2(s, s);
                 if (!mbar_wait(&acc_full[acc], acc_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_ACC)) {
                     ok = false;
@@ -546,7 +572,10 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
                 if (lane == 0) mbar_arrive_cluster(leader_empty + acc * 8u);
                 acc ^= 1u;
                 acc_ph ^= acc ^ 1u;
-                if (++slot == (uint32_t)kPairSlots) { slot = 0; slot_ph ^= 1u; }
+                if (g == kPairGroup - 1 || kb + 1 == kb_total) {  // done with the group's scales
+                    if (lane == 0) mbar_arrive(&sc_empty[slot]);
+                    if (++slot == (uint32_t)kPairSlots) { slot = 0; slot_ph ^= 1u; }
+                }
                 add_scaled32(sum + 48, v1, s2);
             }
             if (!ok) break;

@@ -206,12 +206,12 @@ int launch_glu_backward(const Fp8QuantArgs& a, cudaStream_t stream);
 struct Fp8GemmArgs {
     CUtensorMap tm_w;        // u8 [mats][n][k] of the weight, box 128 x 128, 128-byte swizzle
     CUtensorMap tm_x;        // u8 [rows][contraction] of the tokens, box 128 x token tile, 128-byte swizzle
-    const float* x_scale;    // [contraction blocks, lds]
+    CUtensorMap tm_s;        // f32 [contraction blocks][rows] of the token scales, box 4 x token tile (256: 2 x 128)
     const float* w_scale;    // [mats, ceil(n / 128), ceil(k / 128)]
     const int32_t* counts;   // [mats], or null: one matrix, all rows
     const int32_t* offsets;  // [mats + 1]
     void* out;               // [rows, ldo]
-    int rows, lds, ldo, mats, out_features, contraction, out_dtype, num_sms;
+    int rows, ldo, mats, out_features, contraction, out_dtype, num_sms;
     int out_vec;             // out's rows are 16-byte aligned
     int split;               // set by the launcher: CTAs that share a tile's contraction
 };
