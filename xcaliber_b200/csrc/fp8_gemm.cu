@@ -583,12 +583,12 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
             const int rows = min(32, t.count - t.nt_idx * 256 - (m - lane));  // this warp's live rows (may be <= 0)
             if (rows > 0 && f < a.out_features) {
                 OT* dst = reinterpret_cast<OT*>(a.out) + (size_t)(t.row0 + m - lane) * a.ldo + f;
-                if (a.out_vec && f + 128 <= a.out_features) {
-                    constexpr int kVec = 16 / sizeof(OT), kChunk = 4 * kVec;
-                    // 16-byte piece p of row r sits at piece p ^ (r / 2) & 3: neither side meets a bank conflict
-                    uint8_t* tile = out_tiles + (warp - 4) * kOutBytes;
+                constexpr int kVec = 16 / sizeof(OT), kChunk = 4 * kVec;
+                // 16-byte piece p of row r sits at piece p ^ (r / 2) & 3: neither side meets a bank conflict
+                uint8_t* tile = out_tiles + (warp - 4) * kOutBytes;
 #pragma unroll
-                    for (int c = 0; c < 128; c += kChunk) {
+                for (int c = 0; c < 128; c += kChunk) {
+                    if (a.out_vec && f + c + kChunk <= a.out_features) {
 #pragma unroll
                         for (int p = 0; p < 4; ++p) {
                             Pack<OT, kVec> o;
@@ -607,11 +607,11 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
                             if (r < rows) *reinterpret_cast<uint4*>(dst + (size_t)r * a.ldo + c + p * kVec) = o;
                         }
                         __syncwarp();
-                    }
-                } else if (live) {
+                    } else if (live) {
 #pragma unroll
-                    for (int j = 0; j < 128; ++j)
-                        if (f + j < a.out_features) dst[(size_t)lane * a.ldo + j] = from_f32<OT>(j & 1 ? sum[j / 2].y : sum[j / 2].x);
+                        for (int j = c; j < c + kChunk; ++j)
+                            if (f + j < a.out_features) dst[(size_t)lane * a.ldo + j] = from_f32<OT>(j & 1 ? sum[j / 2].y : sum[j / 2].x);
+                    }
                 }
             }
         }

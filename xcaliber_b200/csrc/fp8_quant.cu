@@ -221,13 +221,23 @@ __global__ __launch_bounds__(kThreads) void fp8_quant_kernel(const Fp8QuantArgs 
         float scale;
         quantise16(v, m, code, scale);
         if (!on) continue;
-        for (int s = 0; s < (SORTED ? a.k : 1); ++s) {
-            const int r = SORTED ? a.topk_row[(size_t)t * a.idx_stride + s] : t;
-            if (SORTED && (r < 0 || r >= a.num_rows)) continue;
-            uint8_t* q = a.q + (size_t)r * a.ldq;
-            store_codes(q, col, a.cols, code);
-            store_codes(q, col + 64, a.cols, code + 2);
-            if (lane == 0) a.scale[(size_t)kb * a.lds + r] = scale;
+        const int32_t* idx = a.topk_row + (size_t)t * a.idx_stride;
+        for (int s0 = 0; s0 < (SORTED ? a.k : 1); s0 += 8) {
+            int rows[SORTED ? 8 : 1];  // loaded together: the stores do not wait for one index after the other
+#pragma unroll
+            for (int s = 0; s < (SORTED ? 8 : 1); ++s) {
+                rows[s] = SORTED ? (s0 + s < a.k ? idx[s0 + s] : -1) : t;
+                if (SORTED && rows[s] >= a.num_rows) rows[s] = -1;
+            }
+#pragma unroll
+            for (int s = 0; s < (SORTED ? 8 : 1); ++s) {
+                const int r = rows[s];
+                if (SORTED && r < 0) continue;
+                uint8_t* q = a.q + (size_t)r * a.ldq;
+                store_codes(q, col, a.cols, code);
+                store_codes(q, col + 64, a.cols, code + 2);
+                if (lane == 0) a.scale[(size_t)kb * a.lds + r] = scale;
+            }
         }
     }
 }

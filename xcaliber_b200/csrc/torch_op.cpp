@@ -226,6 +226,14 @@ void unpermute_cuda(const at::Tensor& rows, const at::Tensor& topk_row, const c1
              "xmoe_unpermute");
 }
 
+// Forms that allocate their result: for decode-sized calls the allocation in Python costs as much as the kernel.
+at::Tensor unpermute_new_cuda(const at::Tensor& rows, const at::Tensor& topk_row, const c10::optional<at::Tensor>& weights) {
+    TORCH_CHECK(rows.dim() == 2 && topk_row.dim() == 2, "rows and topk_row must be matrices");
+    at::Tensor y = at::empty({topk_row.size(0), rows.size(1)}, rows.options());
+    unpermute_cuda(rows, topk_row, weights, y);
+    return y;
+}
+
 void unpermute_backward_cuda(const at::Tensor& dy, const at::Tensor& rows, const at::Tensor& topk_row,
                              const c10::optional<at::Tensor>& weights, at::Tensor& drows, at::Tensor& dw) {
     check_matrix(dy, dy, "dy");
@@ -424,6 +432,13 @@ void fp8_matmul_cuda(const at::Tensor& x, const at::Tensor& x_scale, const at::T
                      bool transpose, at::Tensor& out) {
     fp8_product(x, x_scale, w, w_scale, nullptr, transpose, 0, out);
 }
+at::Tensor fp8_matmul_new_cuda(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w, const at::Tensor& w_scale,
+                               bool transpose, at::ScalarType out_dtype) {
+    TORCH_CHECK(x.dim() == 2 && w.dim() == 2, "x and w must be matrices");
+    at::Tensor out = at::empty({x.size(0), w.size(transpose ? 1 : 0)}, x.options().dtype(out_dtype));
+    fp8_product(x, x_scale, w, w_scale, nullptr, transpose, 0, out);
+    return out;
+}
 void fp8_grouped_matmul_cuda(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w, const at::Tensor& w_scale,
                              const at::Tensor& counts, const at::Tensor& offsets, bool transpose, int64_t rows_in_use,
                              at::Tensor& out) {
@@ -431,7 +446,14 @@ void fp8_grouped_matmul_cuda(const at::Tensor& x, const at::Tensor& x_scale, con
     fp8_product(x, x_scale, w, w_scale, &g, transpose, rows_in_use, out);
 }
 
-// Fake tensors: every result is a tensor of the caller, so there is nothing to shape.
+// Fake tensors: where every result is a tensor of the caller there is nothing to shape.
+at::Tensor unpermute_new_meta(const at::Tensor& rows, const at::Tensor& topk_row, const c10::optional<at::Tensor>&) {
+    return at::empty({topk_row.size(0), rows.size(1)}, rows.options());
+}
+at::Tensor fp8_matmul_new_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor& w, const at::Tensor&, bool transpose,
+                               at::ScalarType out_dtype) {
+    return at::empty({x.size(0), w.size(transpose ? 1 : 0)}, x.options().dtype(out_dtype));
+}
 void permute_meta(const at::Tensor&, const at::Tensor&, at::Tensor&) {}
 void unpermute_meta(const at::Tensor&, const at::Tensor&, const c10::optional<at::Tensor>&, at::Tensor&) {}
 void unpermute_backward_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const c10::optional<at::Tensor>&,
@@ -458,6 +480,9 @@ TORCH_LIBRARY(xmoe_b200, m) {
     m.def("build_info() -> str", &build_info);
     m.def("permute(Tensor x, Tensor topk_row, Tensor(a!) rows) -> ()");
     m.def("unpermute(Tensor rows, Tensor topk_row, Tensor? weights, Tensor(a!) y) -> ()");
+    m.def("unpermute_new(Tensor rows, Tensor topk_row, Tensor? weights) -> Tensor");
+    m.def(
+        "fp8_matmul_new(Tensor x, Tensor x_scale, Tensor w, Tensor w_scale, bool transpose, ScalarType out_dtype) -> Tensor");
     m.def(
         "unpermute_backward(Tensor dy, Tensor rows, Tensor topk_row, Tensor? weights, Tensor(a!) drows, Tensor(b!) dw) "
         "-> ()");
@@ -480,6 +505,8 @@ TORCH_LIBRARY_IMPL(xmoe_b200, CUDA, m) {
     m.impl("repack_gptq", &repack_gptq_cuda);
     m.impl("prep_nvfp4_sf", &prep_nvfp4_sf_cuda);
     m.impl("permute", &permute_cuda);
+    m.impl("unpermute_new", &unpermute_new_cuda);
+    m.impl("fp8_matmul_new", &fp8_matmul_new_cuda);
     m.impl("unpermute", &unpermute_cuda);
     m.impl("unpermute_backward", &unpermute_backward_cuda);
     m.impl("fp8_quant", &fp8_quant_cuda);
@@ -495,6 +522,8 @@ TORCH_LIBRARY_IMPL(xmoe_b200, Meta, m) {
     m.impl("repack_gptq", &repack_gptq_meta);
     m.impl("prep_nvfp4_sf", &prep_nvfp4_sf_meta);
     m.impl("permute", &permute_meta);
+    m.impl("unpermute_new", &unpermute_new_meta);
+    m.impl("fp8_matmul_new", &fp8_matmul_new_meta);
     m.impl("unpermute", &unpermute_meta);
     m.impl("unpermute_backward", &unpermute_backward_meta);
     m.impl("fp8_quant", &fp8_quant_meta);

@@ -54,8 +54,7 @@ def quant(x: torch.Tensor, topk_row: torch.Tensor | None = None, num_rows: int |
             raise RuntimeError("quant into sorted rows needs num_rows or out")
         else:
             out = _zero_rows(num_rows, x.shape[1], x.device)
-    torch_ops.load()
-    torch.ops.xmoe_b200.fp8_quant(x, topk_row, out[0], out[1])
+    torch_ops.op("fp8_quant")(x, topk_row, out[0], out[1])
     return out
 
 
@@ -65,8 +64,7 @@ def quant_weight(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     e, n, k = w3.shape
     codes = torch.zeros(e, n, _up(k, 16), dtype=torch.uint8, device=w.device).view(torch.float8_e4m3fn)[:, :, :k]
     scale = torch.empty(e, _up(n, BLOCK) // BLOCK, _up(k, BLOCK) // BLOCK, dtype=torch.float32, device=w.device)
-    torch_ops.load()
-    torch.ops.xmoe_b200.fp8_quant_weight(w3, codes, scale)
+    torch_ops.op("fp8_quant_weight")(w3, codes, scale)
     return (codes, scale) if w.dim() == 3 else (codes[0], scale[0])
 
 
@@ -88,8 +86,7 @@ def glu_quant(h: torch.Tensor, activation: str = "silu", alpha: float = 1.702, l
     i = h.shape[1] // 2
     if out is None:
         out = empty_rows(h.shape[0], i, h.device) if counts is None else _zero_rows(h.shape[0], i, h.device)
-    torch_ops.load()
-    torch.ops.xmoe_b200.glu_fp8_quant(h, _ACT[activation], alpha, limit, counts, offsets, out[0], out[1])
+    torch_ops.op("glu_fp8_quant")(h, _ACT[activation], alpha, limit, counts, offsets, out[0], out[1])
     return out
 
 
@@ -99,8 +96,7 @@ def glu_backward(da: torch.Tensor, h: torch.Tensor, activation: str = "silu", al
     """The gradient of h from the gradient da [R, I] of the activation (taken as not quantised)."""
     if out is None:
         out = torch.empty_like(h) if counts is None else torch.zeros_like(h)
-    torch_ops.load()
-    torch.ops.xmoe_b200.glu_backward(da, h, _ACT[activation], alpha, limit, counts, offsets, out)
+    torch_ops.op("glu_backward")(da, h, _ACT[activation], alpha, limit, counts, offsets, out)
     return out
 
 
@@ -110,9 +106,8 @@ def matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: tor
     input through the same stored weight). Every 128-block's product is taken from the tensor core and added in fp32 with
     its two scales. Scales of another layout than quant's are laid out anew on every call."""
     if out is None:
-        out = torch.empty(x.shape[0], w.shape[-1 if transpose else -2], dtype=out_dtype, device=x.device)
-    torch_ops.load()
-    torch.ops.xmoe_b200.fp8_matmul(x, x_scale, w, w_scale, transpose, out)
+        return torch_ops.op("fp8_matmul_new")(x, x_scale, w, w_scale, transpose, out_dtype)
+    torch_ops.op("fp8_matmul")(x, x_scale, w, w_scale, transpose, out)
     return out
 
 
@@ -124,8 +119,7 @@ def grouped_matmul(rows: torch.Tensor, row_scale: torch.Tensor, w: torch.Tensor,
     rows). `out` keeps the rows outside the segments; without it they are zero."""
     if out is None:
         out = torch.zeros(rows.shape[0], w.shape[-1 if transpose else -2], dtype=out_dtype, device=rows.device)
-    torch_ops.load()
-    torch.ops.xmoe_b200.fp8_grouped_matmul(rows, row_scale, w, w_scale, counts, offsets, transpose, rows_in_use, out)
+    torch_ops.op("fp8_grouped_matmul")(rows, row_scale, w, w_scale, counts, offsets, transpose, rows_in_use, out)
     return out
 
 

@@ -405,8 +405,7 @@ def permute(x: torch.Tensor, topk_row: torch.Tensor, num_rows: int | None = None
         out = torch.zeros(num_rows, x.shape[-1], dtype=x.dtype, device=x.device)
     elif torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
         raise RuntimeError("permute into `out` is not differentiable: leave out away")
-    torch_ops.load()
-    torch.ops.xmoe_b200.permute(x, topk_row, out)
+    torch_ops.op("permute")(x, topk_row, out)
     return out
 
 
@@ -425,9 +424,8 @@ def unpermute(rows: torch.Tensor, topk_row: torch.Tensor, weights: torch.Tensor 
             raise RuntimeError("unpermute into `out` is not differentiable: leave out away")
         return _Unpermute.apply(rows, topk_row, weights)
     if out is None:
-        out = torch.empty(topk_row.shape[0], rows.shape[-1], dtype=rows.dtype, device=rows.device)
-    torch_ops.load()
-    torch.ops.xmoe_b200.unpermute(rows, topk_row, weights, out)
+        return torch_ops.op("unpermute_new")(rows, topk_row, weights)
+    torch_ops.op("unpermute")(rows, topk_row, weights, out)
     return out
 
 
@@ -438,8 +436,7 @@ def unpermute_backward(dy: torch.Tensor, rows: torch.Tensor, topk_row: torch.Ten
     they are zero. No row may be named twice."""
     drows = torch.zeros_like(rows) if out is None else out
     dw = torch.empty(topk_row.shape, dtype=torch.float32, device=dy.device)
-    torch_ops.load()
-    torch.ops.xmoe_b200.unpermute_backward(dy, rows, topk_row, weights, drows, dw)
+    torch_ops.op("unpermute_backward")(dy, rows, topk_row, weights, drows, dw)
     return drows, dw
 
 

@@ -28,6 +28,18 @@ def load() -> None:
     _loaded = True
 
 
+_ops: dict = {}
+
+
+def op(name: str):
+    """The registered op `name`, without the lookups of torch.ops (they cost as much as a small kernel)."""
+    found = _ops.get(name)
+    if found is None:
+        load()
+        found = _ops[name] = getattr(torch.ops.xmoe_b200, name).default
+    return found
+
+
 def cfg_lists(cfg) -> tuple[list[int], list[float]]:
     """The int and float fields of an XMoEConfig, in declaration order, as the op takes them."""
     ints = [int(getattr(cfg, name)) for name, ctype in cfg._fields_[:12]]
