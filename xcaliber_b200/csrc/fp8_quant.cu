@@ -205,8 +205,8 @@ template <typename T, bool VEC, bool SORTED>
 __global__ __launch_bounds__(kThreads) void fp8_quant_kernel(const Fp8QuantArgs a, int kb_total, int share) {
     const int unit = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
     const T* x = reinterpret_cast<const T*>(a.x);
-    const size_t first = (size_t)blockIdx.x * share + unit;
-    Walk w{(int)(first / kb_total), (int)(first % kb_total)};
+    const uint32_t first = blockIdx.x * (uint32_t)share + unit;  // 2^32 blocks of 128 values would not fit the memory
+    Walk w{(int)(first / (uint32_t)kb_total), (int)(first % (uint32_t)kb_total)};
     const int d_row = kUnits / kb_total, d_kb = kUnits % kb_total;
     // every group takes the same number of steps (the shuffles need all lanes of a warp): a block past the last row loads
     // and stores nothing
@@ -217,27 +217,27 @@ __global__ __launch_bounds__(kThreads) void fp8_quant_kernel(const Fp8QuantArgs 
         const int cols = on ? a.cols : 0;
         float v[16];
         const float m = max_nan(load8<T, VEC>(row, col, cols, v), load8<T, VEC>(row, col + 64, cols, v + 8));
+        // a sorted row's slots, one per lane, on their way while the block is quantised
+        const int32_t* idx = a.topk_row + (size_t)(on ? t : 0) * a.idx_stride;
+        int mine = SORTED && lane < a.k ? idx[lane] : -1;
         uint32_t code[4];
         float scale;
         quantise16(v, m, code, scale);
-        if (!on) continue;
-        const int32_t* idx = a.topk_row + (size_t)t * a.idx_stride;
-        for (int s0 = 0; s0 < (SORTED ? a.k : 1); s0 += 8) {
-            int rows[SORTED ? 8 : 1];  // loaded together: the stores do not wait for one index after the other
-#pragma unroll
-            for (int s = 0; s < (SORTED ? 8 : 1); ++s) {
-                rows[s] = SORTED ? (s0 + s < a.k ? idx[s0 + s] : -1) : t;
-                if (SORTED && rows[s] >= a.num_rows) rows[s] = -1;
-            }
-#pragma unroll
-            for (int s = 0; s < (SORTED ? 8 : 1); ++s) {
-                const int r = rows[s];
-                if (SORTED && r < 0) continue;
-                uint8_t* q = a.q + (size_t)r * a.ldq;
-                store_codes(q, col, a.cols, code);
-                store_codes(q, col + 64, a.cols, code + 2);
-                if (lane == 0) a.scale[(size_t)kb * a.lds + r] = scale;
-            }
+        auto store = [&](int r) {
+            uint8_t* q = a.q + (size_t)r * a.ldq;
+            store_codes(q, col, a.cols, code);
+            store_codes(q, col + 64, a.cols, code + 2);
+            if (lane == 0) a.scale[(size_t)kb * a.lds + r] = scale;
+        };
+        if (!SORTED) {
+            if (on) store(t);
+            continue;
+        }
+#pragma unroll 1
+        for (int s = 0; s < a.k; ++s) {
+            if (s && s % kLanes == 0) mine = s + lane < a.k ? idx[s + lane] : -1;
+            const int r = __shfl_sync(0xffffffffu, mine, s % kLanes, kLanes);
+            if (on && r >= 0 && r < a.num_rows) store(r);
         }
     }
 }
@@ -283,7 +283,7 @@ __device__ __forceinline__ void glu_gradient(float g, float u, float da, float a
 // neither read nor written. The live rows are numbered through; every CTA takes an equal, contiguous share of their blocks
 // and finds its first expert once.
 template <typename T, bool VEC, int ACT, bool BACKWARD>
-__global__ __launch_bounds__(kThreads, BACKWARD ? 1 : 4) void glu_kernel(const Fp8QuantArgs a, int kb_total) {
+__global__ __launch_bounds__(kThreads, BACKWARD ? 5 : 4) void glu_kernel(const Fp8QuantArgs a, int kb_total) {
     // the gradient has no block to share a scale: 16 lanes with 8 values, for more warps in flight
     constexpr int kP = BACKWARD ? 1 : 2, kLanes = 16 / kP, kUnits = kThreads / kLanes;
     __shared__ int before[kMaxMats + 1];  // live rows of the experts before e
