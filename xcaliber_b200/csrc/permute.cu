@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kThreads) void unpermute_kernel(const T* __restrict
 // One CTA per token: dy[t] is read once per batch of slots, every thread keeps one partial dot product per slot, and
 // the partials are added over the warp and then over the warps in a fixed order.
 template <typename T, int VEC, int WT, int SLOTS>
-__global__ __launch_bounds__(kThreads) void unpermute_backward_kernel(const T* __restrict__ dy, const T* __restrict__ rows,
+__global__ __launch_bounds__(kThreads, 3) void unpermute_backward_kernel(const T* __restrict__ dy, const T* __restrict__ rows,
                                                                       const int32_t* __restrict__ topk_row,
                                                                       const void* __restrict__ w, T* __restrict__ drows,
                                                                       float* __restrict__ dw, int n, int hv, int k,
