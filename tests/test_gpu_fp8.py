@@ -357,6 +357,40 @@ def test_grouped_matmul_keeps_to_its_buffers():
     assert fp8.status() == 0 and bool((y[10:] == -7.0).all()) and not bool((y[:10] == -7.0).all())
 
 
+def test_glu_keeps_to_its_buffers():
+    """As the products: segments outside the rows are empty, one past the end is cut, negative counts are none."""
+    h = torch.randn(64, 256, device="cuda").bfloat16()
+    whole = fp8.glu_quant(h)
+    counts = torch.tensor([10, 5, 2 ** 30, -7, 2 ** 31 - 1, 3], dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([0, -16, 48, 16, 4096, 2 ** 31 - 8, 0], dtype=torch.int32, device="cuda")
+    out = fp8.empty_rows(64, 128, "cuda")
+    out[0].view(torch.uint8).fill_(0x21)
+    out[1].fill_(-1.0)
+    fp8.glu_quant(h, counts=counts, offsets=offsets, out=out)
+    live = torch.zeros(64, dtype=torch.bool, device="cuda")
+    live[:10] = live[48:] = True
+    assert torch.equal(out[0].view(torch.uint8)[live], whole[0].view(torch.uint8)[live]) and torch.equal(out[1][live], whole[1][live])
+    assert bool((out[0].view(torch.uint8)[~live] == 0x21).all()) and bool((out[1][~live] == -1.0).all())
+    da = torch.randn(64, 128, device="cuda").bfloat16()
+    dh = fp8.glu_backward(da, h, counts=counts, offsets=offsets, out=torch.full_like(h, 3.0))
+    assert torch.equal(dh[live], fp8.glu_backward(da, h)[live]) and bool((dh[~live] == 3.0).all())
+
+
+def test_overlapping_segments_beyond_what_can_be_counted():
+    """1024 experts that all claim the same 2^19 rows: more tiles than 31 bits hold. Reported, nothing is written."""
+    r, e, n = 2 ** 19, 1024, 8192
+    codes = torch.zeros(r, 16, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    scale = torch.zeros(1, r, device="cuda").t()
+    w = torch.zeros(n, 16, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)[None].expand(e, n, 16)
+    counts = torch.full((e,), r, dtype=torch.int32, device="cuda")
+    offsets = torch.zeros(e + 1, dtype=torch.int32, device="cuda")
+    out = torch.full((r, n), 7.0, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError):  # matrices that lie on top of one another are refused
+        fp8.grouped_matmul(codes, scale, w, torch.ones(e, n // 128, 1, device="cuda"), counts, offsets, rows_in_use=16, out=out)
+    fp8.grouped_matmul(codes, scale, w.contiguous(), torch.ones(e, n // 128, 1, device="cuda"), counts, offsets, rows_in_use=16, out=out)
+    assert fp8.status() == 0x700 and bool((out == 7.0).all())
+
+
 def test_rows_far_behind_in_a_large_buffer():
     """Offsets beyond 2^31 elements, in codes, outputs and sorted rows."""
     k, r = 8192, 2 ** 18 + 256

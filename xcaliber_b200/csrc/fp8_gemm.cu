@@ -68,6 +68,15 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     return d;
 }
 
+// The number of tiles, by all threads; none (and reported) if segments that overlap make more than 31 bits can count.
+__device__ __forceinline__ int count_tiles(const int* prefix, int mats, int threads) {
+    int bad = 0;
+    for (int e = threadIdx.x; e < mats; e += threads) bad |= prefix[e + 1] < prefix[e];
+    if (!__syncthreads_or(bad)) return prefix[mats];
+    if (threadIdx.x == 0) atomicCAS(&g_fp8_status, 0u, kBadSegment);
+    return 0;
+}
+
 __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
 }
@@ -179,7 +188,7 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const int total_tiles = prefix[a.mats];
+    const int total_tiles = count_tiles(prefix, a.mats, C::kThreads);
     // a.split > 1: the CTAs of a cluster share one tile, each takes a part of the contraction (a cluster per tile at most)
     const int split = a.split, rank = split > 1 ? (int)cluster_ctarank() : 0;
     const int kb_lo = kb_total * rank / split, kb_hi = kb_total * (rank + 1) / split;
@@ -442,7 +451,7 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const int total_tiles = prefix[a.mats];
+    const int total_tiles = count_tiles(prefix, a.mats, kPairThreads);
     const int stride = balanced_stride(total_tiles, (int)gridDim.x >> 1);
     const int first = ((int)blockIdx.x >> 1) < stride ? (int)blockIdx.x >> 1 : total_tiles;
 

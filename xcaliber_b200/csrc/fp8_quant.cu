@@ -287,18 +287,19 @@ __global__ __launch_bounds__(kThreads, BACKWARD ? 5 : 4) void glu_kernel(const F
     // the gradient has no block to share a scale: 16 lanes with 8 values, for more warps in flight
     constexpr int kP = BACKWARD ? 1 : 2, kLanes = 16 / kP, kUnits = kThreads / kLanes;
     __shared__ int before[kMaxMats + 1];  // live rows of the experts before e
-    __shared__ int shift[kMaxMats];       // buffer row - live row, within expert e
+    __shared__ int shift[kMaxMats];       // the experts' counts, then: buffer row - live row, within expert e
     const int mats = a.counts ? a.e_tot : 1;
-    if (a.counts) {
-        if (threadIdx.x < 32) tile_prefix_build(before, a.counts, mats, 1, 1);
-    } else if (threadIdx.x == 0) {
-        before[0] = 0;
-        before[1] = a.rows;
+    // segments are kept inside the rows: one that starts outside counts as empty, one that runs past the end is cut
+    for (int e = threadIdx.x; e < mats; e += kThreads) {
+        const int c = a.counts ? a.counts[e] : a.rows, o = a.counts ? a.offsets[e] : 0;
+        shift[e] = o < 0 || o >= a.rows ? 0 : max(min(c, a.rows - o), 0);
     }
+    __syncthreads();
+    if (threadIdx.x < 32) tile_prefix_build(before, shift, mats, 1, 1);
     __syncthreads();
     for (int e = threadIdx.x; e < mats; e += kThreads) shift[e] = (a.counts ? a.offsets[e] : 0) - before[e];
     __syncthreads();
-    const int live = before[mats];
+    const int live = max(before[mats], 0);
     const size_t blocks = (size_t)live * kb_total;
     const size_t share = ((blocks + gridDim.x - 1) / gridDim.x + kUnits - 1) / kUnits * kUnits;
     const size_t begin = blockIdx.x * share;
