@@ -8,6 +8,11 @@
 // One block of 128 is handled by 8 lanes with twice 8 values each: two coalesced 16-byte loads per lane (bf16, fp16), three
 // shuffles for the maximum, two 8-byte stores. Scales are stored block-major, [ceil(cols / 128), lds], the order in which the product
 // reads them: the scales of consecutive rows for one block are contiguous.
+//
+// Bound by instructions rather than bytes where the input has 16 bits: about 15 per value of which 8 are on the half-rate
+// integer pipe (unpacking, maxima, conversions), and ties of two codes, which bf16 values with a bf16 maximum meet in one
+// block of 14, cost a branch. Measured: fp32 8192 x 4096 31 us = 5.5 TB/s, bf16 8192 x 7168 55 us = 3.2 TB/s, gated
+// activation of 16384 rows of 2 x 2880 60 to 71 us = 3.4 to 4.0 TB/s, its gradient 100 to 119 us = 4.0 to 4.7 TB/s.
 #include "elem.cuh"
 #include "kernels.h"
 #include "tile_sched.cuh"
