@@ -676,7 +676,9 @@ int launch_cluster(void (*kernel)(Fp8GemmArgs), const Fp8GemmArgs& a, unsigned g
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
+    if (cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess) return XMOE_OK;
+    cudaGetLastError();  // reported here: the next call does not find it again
+    return XMOE_ERR_CUDA;
 }
 
 template <bool TRANS, typename OT>
