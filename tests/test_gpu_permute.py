@@ -131,6 +131,23 @@ def test_route_pack_is_the_layers_permutation_and_drops_slots():
     assert bool((r.topk_w[:, k] == 1).all()) and r.rows_in_use == n * (k + 1) and int(r.offsets[-1]) <= r.num_rows
 
 
+@pytest.mark.parametrize("n", [1, 40, 700])  # one and several chunks of the kernel
+def test_route_pack_gives_every_slot_a_row_of_its_own(n):
+    """An expert named in several slots of a token: as many rows, in slot order, behind those of the tokens before."""
+    g = torch.Generator().manual_seed(n)
+    e, k = 4, 6
+    idx = torch.randint(-1, e, (n, k), generator=g, dtype=torch.int32)
+    idx[0] = 2
+    r = ops.route_pack(idx.cuda(), torch.rand(n, k, generator=g).bfloat16().cuda(), e)
+    assert int(r.status[0]) == 0 and r.counts.tolist() == [int((idx == x).sum()) for x in range(e)]
+    want = torch.full((n, k), -1, dtype=torch.int32)
+    for x in range(e):
+        t, s = torch.nonzero(idx == x, as_tuple=True)  # token by token, slot by slot
+        want[t, s] = int(r.offsets[x]) + torch.arange(len(t), dtype=torch.int32)
+        assert torch.equal(r.row_token.cpu()[int(r.offsets[x]):int(r.offsets[x]) + len(t)], t.int())
+    assert torch.equal(r.topk_row.cpu(), want)
+
+
 def test_plan_strides_rows_outside_streams_and_empty_calls():
     n, k, h = 50, 2, 256
     row, _, _, r = P.plan(n, 8, k, seed=5)
@@ -195,3 +212,33 @@ def test_gradients_in_a_captured_graph():
         want = step(new[0].requires_grad_(), new[1].requires_grad_(), new[2])
         for a, b in zip(got, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("what", ["plan type", "plan shape", "plan device", "strides", "type", "width", "weights shape", "weights type"])
+def test_refusals(what):
+    row, _, _, r = P.plan(6, 4, 2, seed=1)
+    plan = row.cuda()
+    rows, w, y = torch.randn(r, 64, device="cuda"), torch.rand(6, 2, device="cuda"), torch.empty(6, 64, device="cuda")
+    if what == "plan type":
+        plan = plan.long()
+    elif what == "plan shape":
+        plan = plan[:5]
+    elif what == "plan device":
+        plan = row
+    elif what == "strides":
+        rows = torch.randn(r, 128, device="cuda")[:, ::2]
+    elif what == "type":
+        rows = rows.double()
+    elif what == "width":
+        rows = rows[:, :32].contiguous()
+    elif what == "weights shape":
+        w = w[:, :1]
+    else:
+        w = w.half()
+    with pytest.raises(RuntimeError):
+        ops.unpermute(rows, plan, w, out=y)
+    with pytest.raises(RuntimeError):
+        ops.unpermute_backward(y, rows, plan, w)
+    if not what.startswith("weights"):
+        with pytest.raises(RuntimeError):
+            ops.permute(y, plan, out=rows)

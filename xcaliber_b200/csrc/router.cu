@@ -201,9 +201,16 @@ __global__ __launch_bounds__(256) void route_scatter_kernel(
             }
             // a caller slot is valid under the same test as the histograms (ids in [E, e_tot) belong to the
             // shared experts' own slots and were never counted for a caller slot)
-            if (e >= 0 && e < (lane < topk ? E : e_tot)) {
-                const int p = warp_base[warp][e];
-                warp_base[warp][e] = p + 1;
+            const bool valid = e >= 0 && e < (lane < topk ? E : e_tot);
+            // a caller may name an expert in several slots of a token: they take consecutive rows in slot order (and were
+            // counted one by one)
+            const unsigned slots = k_eff < 32 ? (1u << k_eff) - 1u : 0xffffffffu;
+            const unsigned same = __match_any_sync(slots, valid ? e : -1 - lane);
+            const int rank = __popc(same & ((1u << lane) - 1u));
+            const int p = valid ? warp_base[warp][e] + rank : -1;
+            __syncwarp(slots);
+            if (valid) {
+                if (rank == 0) warp_base[warp][e] = p + __popc(same);
                 const int r = start[e] + p;
                 topk_off[(size_t)t * idx_stride + lane] = p;
                 topk_row[(size_t)t * idx_stride + lane] = r;
