@@ -493,6 +493,43 @@ def test_layer_forward_and_gradients(name, n):
     assert fp8.status() == 0
 
 
+def test_layer_with_an_expert_twice_and_with_nothing():
+    """A token may name an expert twice (two slots, two rows, weights add up); a batch may have no slot left at all."""
+    shape = SHAPES["flat"]
+    layer = _layer(shape)
+    torch.manual_seed(9)
+    n = 37
+    x = torch.randn(n, shape.hidden, device="cuda").bfloat16().requires_grad_()
+    w = torch.rand(n, 2, device="cuda").requires_grad_()
+    dy = torch.randn(n, shape.hidden, device="cuda").bfloat16()
+    twice = torch.randint(0, shape.num_experts, (n, 1), device="cuda", dtype=torch.int32).expand(n, 2).contiguous()
+    y = layer.forward_routed(x, twice, w)
+    gx, gw = torch.autograd.grad(y, (x, w), dy)
+    ry, rx, rw = _layer_plain(layer, x.detach(), twice, w.detach(), dy)
+    assert _far(y, ry) <= FORWARD and _far(gx, rx) <= BACKWARD and _far(gw, rw) <= BACKWARD
+    none = torch.full((n, 2), -1, dtype=torch.int32, device="cuda")
+    y = layer.forward_routed(x, none, w)
+    gx, gw = torch.autograd.grad(y, (x, w), dy)
+    assert not y.any() and not gx.any() and not gw.any() and fp8.status() == 0
+
+
+def test_products_in_flight_together():
+    """Large and small products (CTA pairs, clusters that share a tile, plain CTAs) on three streams at once."""
+    jobs = [_operands(700, 2048, 1024, seed=1), _operands(3, 512, 4096, seed=2), _operands(40, 3000, 512, seed=3)]
+    want = [fp8.matmul(*x, *w) for x, w in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    got = [[] for _ in jobs]
+    for _ in range(20):
+        for (x, w), s, g in zip(jobs, streams, got):
+            with torch.cuda.stream(s):
+                g.append(fp8.matmul(*x, *w))
+    torch.cuda.synchronize()
+    for g, ref in zip(got, want):
+        assert all(torch.equal(y, ref) for y in g)
+    assert fp8.status() == 0
+
+
 def test_layer_on_another_stream_and_in_two_graphs():
     """Two captured graphs of the same layer and an eager call, in flight together, do not disturb one another."""
     shape = SHAPES["flat"]
