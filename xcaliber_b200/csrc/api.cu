@@ -536,6 +536,7 @@ int forward_impl(const xmoe_config* cfg, const xmoe_weights* w, const void* x, c
     }
 
     PackArgs p;
+    p.distinct = ext_idx == nullptr;  // the router names an expert once
     p.topk_idx = topk_idx;
     p.topk_w = topk_w;
     p.N = n;

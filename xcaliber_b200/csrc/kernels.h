@@ -49,6 +49,7 @@ struct PackArgs {
     void* row_weight;    // bf16 [R_cap]
     uint32_t* status;
     const int32_t* n_valid = nullptr;  // optional, device: tokens at and beyond *n_valid are not in use and are not walked
+    bool distinct = false;             // no token names an expert twice (the router's own output)
 };
 
 struct ActScale {  // same meaning as the reference's MoeActScale (preamble.cuh:12-15)

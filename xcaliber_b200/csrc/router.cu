@@ -76,6 +76,7 @@ __global__ __launch_bounds__(256) void route_hist_kernel(const int32_t* __restri
     for (int e = threadIdx.x; e < e_tot; e += blockDim.x) chunk_hist[(size_t)blockIdx.x * e_tot + e] = hist[e];
 }
 
+template <bool CHECK>
 __global__ __launch_bounds__(256) void route_scatter_kernel(
     int32_t* __restrict__ topk_idx, uint16_t* __restrict__ topk_w, int N, int E, int topk, int idx_stride,
     int n_shared, const int32_t* __restrict__ chunk_hist, int n_chunks, int32_t* __restrict__ counts,
@@ -102,14 +103,35 @@ __global__ __launch_bounds__(256) void route_scatter_kernel(
     if (threadIdx.x == 0) carry = 0;
     __syncthreads();
     const int t_mine = chunk * kPackChunk + threadIdx.x;
+    // CHECK (routing of a caller; a router's has none): whether the token names an expert in several slots: 256 bits of the ids seen so far, and beyond 256 experts, where ids
+    // share a bit, a comparison of all pairs
+    unsigned long long seen[4] = {0ull, 0ull, 0ull, 0ull};
+    bool twice = false;
     if (t_mine < N) {
+        const int32_t* mine = topk_idx + (size_t)t_mine * idx_stride;
         for (int k = 0; k < topk; ++k) {
-            const int e = topk_idx[(size_t)t_mine * idx_stride + k];
-            if (e >= 0 && e < E) atomicAdd(&warp_base[warp][e], 1);
-            else if (e != -1) atomicExch(status, 0x600u);  // expert id outside [0, E); -1 = slot not in use
+            const int e = mine[k];
+            if (e >= 0 && e < E) {
+                atomicAdd(&warp_base[warp][e], 1);
+                const unsigned long long bit = 1ull << (e & 63);
+#pragma unroll
+                for (int j = 0; j < (CHECK ? 4 : 0); ++j) {
+                    const unsigned long long b = ((e >> 6) & 3) == j ? bit : 0ull;
+                    twice |= (seen[j] & b) != 0ull;
+                    seen[j] |= b;
+                }
+            } else if (e != -1) {
+                atomicExch(status, 0x600u);  // expert id outside [0, E); -1 = slot not in use
+            }
+        }
+        if (twice && E > 256) {
+            twice = false;
+            for (int k = 1; k < topk; ++k)
+                for (int j = 0; j < k; ++j) twice |= mine[j] == mine[k] && mine[k] >= 0;
         }
         for (int s = 0; s < n_shared; ++s) atomicAdd(&warp_base[warp][E + s], 1);
     }
+    const bool careful = CHECK && __any_sync(0xffffffffu, twice);  // among the 32 tokens that this warp walks below
     __syncthreads();
 
     // totals and this chunk's base (tokens of earlier chunks come first). A single chunk is its own
@@ -172,6 +194,37 @@ __global__ __launch_bounds__(256) void route_scatter_kernel(
     // one dependent global load per step.
     const int k_eff = topk + n_shared;
     const int t_first = chunk * kPackChunk + warp * 32;
+    if (careful) {
+        // The same walk for tokens that name an expert in several slots: those
+        // slots take consecutive rows in slot order, as they were counted one by one.
+        const unsigned slots = k_eff < 32 ? (1u << k_eff) - 1u : 0xffffffffu;
+#pragma unroll 1
+        for (int t = t_first; t < min(t_first + 32, N); ++t) {
+            if (lane < k_eff) {
+                const size_t at = (size_t)t * idx_stride + lane;
+                if (lane >= topk) {
+                    topk_idx[at] = E + (lane - topk);
+                    topk_w[at] = 0x3f80u;  // 1.0 in bf16
+                }
+                const int e = topk_idx[at];
+                const bool valid = e >= 0 && e < (lane < topk ? E : e_tot);
+                const int base = valid ? warp_base[warp][e] : 0;
+                const unsigned same = __match_any_sync(slots, valid ? e : -1 - lane);
+                const int before = __popc(same & ((1u << lane) - 1u));
+                __syncwarp(slots);  // all have read the base: the first slot of an expert moves it on
+                if (valid && before == 0) warp_base[warp][e] = base + __popc(same);
+                const int r = valid ? start[e] + base + before : -1;
+                topk_off[at] = valid ? base + before : -1;
+                topk_row[at] = r;
+                if (valid) {
+                    row_token[r] = t;
+                    row_weight[r] = topk_w[at];
+                }
+            }
+            __syncwarp();
+        }
+        return;
+    }
     int e_pre[32];
     uint16_t w_pre[32];
 #pragma unroll
@@ -201,16 +254,9 @@ __global__ __launch_bounds__(256) void route_scatter_kernel(
             }
             // a caller slot is valid under the same test as the histograms (ids in [E, e_tot) belong to the
             // shared experts' own slots and were never counted for a caller slot)
-            const bool valid = e >= 0 && e < (lane < topk ? E : e_tot);
-            // a caller may name an expert in several slots of a token: they take consecutive rows in slot order (and were
-            // counted one by one)
-            const unsigned slots = k_eff < 32 ? (1u << k_eff) - 1u : 0xffffffffu;
-            const unsigned same = __match_any_sync(slots, valid ? e : -1 - lane);
-            const int rank = __popc(same & ((1u << lane) - 1u));
-            const int p = valid ? warp_base[warp][e] + rank : -1;
-            __syncwarp(slots);
-            if (valid) {
-                if (rank == 0) warp_base[warp][e] = p + __popc(same);
+            if (e >= 0 && e < (lane < topk ? E : e_tot)) {
+                const int p = warp_base[warp][e];
+                warp_base[warp][e] = p + 1;
                 const int r = start[e] + p;
                 topk_off[(size_t)t * idx_stride + lane] = p;
                 topk_row[(size_t)t * idx_stride + lane] = r;
@@ -276,7 +322,8 @@ int launch_route_pack(const PackArgs& a, cudaStream_t stream) {
     if (chunks > 1)  // a single chunk builds its totals inside the scatter kernel
         route_hist_kernel<<<chunks, 256, 0, stream>>>(a.topk_idx, a.N, a.E, a.topk, a.idx_stride, a.n_shared,
                                                       a.chunk_hist, a.n_valid);
-    route_scatter_kernel<<<chunks, 256, 0, stream>>>(a.topk_idx, (uint16_t*)a.topk_w, a.N, a.E, a.topk,
+    auto kernel = a.distinct ? route_scatter_kernel<false> : route_scatter_kernel<true>;
+    kernel<<<chunks, 256, 0, stream>>>(a.topk_idx, (uint16_t*)a.topk_w, a.N, a.E, a.topk,
                                                      a.idx_stride, a.n_shared, a.chunk_hist, chunks, a.counts,
                                                      a.offsets, a.topk_off, a.topk_row, a.row_token,
                                                      (uint16_t*)a.row_weight, a.status, a.n_valid);
