@@ -99,6 +99,21 @@ def test_quant_into_sorted_rows(n, e, k, h, dropped):
     assert torch.equal(out[0].float()[at], sorted_[0].float()[at]) and torch.equal(out[1][at], sorted_[1][at])
 
 
+def test_empty_calls():
+    x = torch.randn(4, 256, device="cuda").bfloat16()
+    none = torch.empty(0, 2, dtype=torch.int32, device="cuda")
+    for codes, scale in (fp8.quant(x[:0]), fp8.quant(x[:0], none, 0), fp8.glu_quant(torch.cat([x, x], 1)[:0])):
+        assert codes.shape == (0, 256) and scale.shape == (0, 2)
+    codes, scale = fp8.quant(x[:0], none, 128)
+    assert codes.shape == (128, 256) and not codes.float().any() and not scale.any()
+    assert fp8.glu_backward(x[:0], torch.cat([x, x], 1)[:0]).shape == (0, 512)
+    codes, scale = fp8.quant_weight(torch.empty(0, 128, 256, device="cuda"))
+    assert codes.shape == (0, 128, 256) and scale.shape == (0, 1, 2)
+    wq = fp8.quant_weight(torch.randn(2, 128, 256, device="cuda"))
+    c, o = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    assert fp8.grouped_matmul(*fp8.quant(x[:0]), *wq, c, o).shape == (0, 128)
+
+
 def test_quant_leaves_the_padding_of_a_row():
     """130 columns lie in rows of 144 bytes: the 14 bytes behind them are not written."""
     x = torch.randn(9, 130, device="cuda")

@@ -291,6 +291,7 @@ int32_t check_scale_out(const at::Tensor& s, int64_t rows, int64_t cols, const a
     TORCH_CHECK(s.is_cuda() && s.device() == like.device() && s.scalar_type() == at::kFloat && s.dim() == 2 &&
                     s.size(0) == rows && s.size(1) == blocks_of(cols),
                 "scale must be fp32 [rows, ceil(cols / 128)]");
+    if (rows == 0) return 0;  // nothing will be written
     const int64_t ld = scale_ld(s);
     TORCH_CHECK(ld >= 0, "scale must be laid out block-major: strides (1, multiple of 4), 16-byte aligned (as fp8.quant lays it out)");
     return i32(ld, "the scales' stride");
