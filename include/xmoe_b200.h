@@ -344,7 +344,8 @@ int xmoe_forward_gated(const xmoe_config* cfg, const xmoe_weights* w, const void
  * entry outside [0, num_rows) is a slot without a row. No two slots name the same row (a plan of xmoe_route_pack never
  * does; xmoe_unpermute alone also takes plans that do). Rows that no slot names are left as they were. Element types:
  * XMOE_BF16 / XMOE_FP16 / XMOE_FP32 for x, y, rows; XMOE_BF16 / XMOE_FP32 for the weights w [n_tokens, w_stride]. Sums in
- * fp32, slot 0 first, rounded once; no atomics. Any hidden size; 16-byte accesses where rows are 16-byte aligned. */
+ * fp32, slot 0 first, rounded once; no atomics. Any hidden size; 16-byte accesses where rows are 16-byte
+ * aligned, else 4-byte ones, else (16-bit types of an odd width) one element at a time. */
 #define XMOE_BF16 0
 #define XMOE_FP16 1
 #define XMOE_FP32 2

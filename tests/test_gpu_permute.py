@@ -26,7 +26,7 @@ def assert_near(got, ref, tol):
 
 CASES = [  # tokens, experts, k, hidden, dropped
     (1, 8, 2, 4096, 0.0), (1, 1, 1, 1, 0.0), (3, 4, 4, 7, 0.0), (17, 8, 3, 2880, 0.3), (64, 128, 8, 2048, 0.0),
-    (33, 16, 9, 136, 0.1), (129, 32, 17, 100, 0.2), (5, 8, 2, 12288, 0.0), (40, 4, 2, 1023, 1.0), (300, 60, 6, 513, 0.05),
+    (33, 16, 9, 136, 0.1), (129, 32, 17, 100, 0.2), (5, 8, 2, 12288, 0.0), (40, 4, 2, 1023, 1.0), (300, 60, 6, 513, 0.05), (21, 8, 2, 2050, 0.0), (9, 8, 8, 4101, 0.1),
 ]
 
 

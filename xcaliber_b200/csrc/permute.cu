@@ -22,28 +22,39 @@ constexpr int kThreads = 256;
 
 // A CTA covers 256 >> shift tokens with 1 << shift threads side by side on each; blockIdx.y walks a wider row. So every
 // thread moves one vector of one token without a division, and few tokens still spread over many CTAs.
+// Where an access is narrow (rows that are not 16-byte aligned) a thread takes REP of them, 1 << shift apart.
 struct Place {
     size_t t;
     int c;
 };
+template <int REP>
 __device__ __forceinline__ Place place(int shift) {
     return {(size_t)blockIdx.x * (kThreads >> shift) + (threadIdx.x >> shift),
-            (int)(((size_t)blockIdx.y << shift) + (threadIdx.x & ((1 << shift) - 1)))};
+            (int)(((size_t)blockIdx.y * REP << shift) + (threadIdx.x & ((1 << shift) - 1)))};
 }
+template <typename T, int VEC> constexpr int kPermuteRep = VEC * sizeof(T) == 16 ? 1 : 4;
+template <typename T, int VEC> constexpr int kUnpermuteRep = VEC * sizeof(T) == 16 ? 1 : 2;
 
 template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void permute_kernel(const T* __restrict__ x, const int32_t* __restrict__ topk_row,
                                                            T* __restrict__ rows, int n, int hv, int k, int idx_stride,
                                                            int num_rows, int shift) {
-    const Place p = place(shift);
+    constexpr int R = kPermuteRep<T, VEC>;
+    const Place p = place<R>(shift);
     if (p.t >= (size_t)n || p.c >= hv) return;
     const size_t h = (size_t)hv * VEC;
-    const Pack<T, VEC> v = load_pack_once<T, VEC>(x + p.t * h + (size_t)p.c * VEC);
+    Pack<T, VEC> v[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u)
+        if (u == 0 || p.c + (u << shift) < hv) v[u] = load_pack_once<T, VEC>(x + p.t * h + (size_t)(p.c + (u << shift)) * VEC);
     const int32_t* idx = topk_row + p.t * idx_stride;
 #pragma unroll 8
     for (int s = 0; s < k; ++s) {
         const int r = idx[s];
-        if (r >= 0 && r < num_rows) store_pack<T, VEC>(rows + (size_t)r * h + (size_t)p.c * VEC, v);
+        if (r < 0 || r >= num_rows) continue;
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+            if (u == 0 || p.c + (u << shift) < hv) store_pack<T, VEC>(rows + (size_t)r * h + (size_t)(p.c + (u << shift)) * VEC, v[u]);
     }
 }
 
@@ -61,16 +72,19 @@ template <typename T, int VEC, int WT, int SLOTS>
 __global__ __launch_bounds__(kThreads) void unpermute_kernel(const T* __restrict__ rows, const int32_t* __restrict__ topk_row,
                                                              const void* __restrict__ w, T* __restrict__ y, int n, int hv,
                                                              int k, int idx_stride, int w_stride, int num_rows, int shift) {
-    const Place p = place(shift);
+    constexpr int R = kUnpermuteRep<T, VEC>;
+    const Place p = place<R>(shift);
     if (p.t >= (size_t)n || p.c >= hv) return;
     const size_t h = (size_t)hv * VEC;
     const int32_t* idx = topk_row + p.t * idx_stride;
-    float acc[VEC];
+    float acc[R][VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    for (int u = 0; u < R; ++u)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[u][j] = 0.f;
     for (int s0 = 0; s0 < k; s0 += SLOTS) {
         int r[SLOTS];
-        Pack<T, VEC> v[SLOTS];
+        Pack<T, VEC> v[R][SLOTS];
         float ws[SLOTS];
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) {
@@ -79,19 +93,28 @@ __global__ __launch_bounds__(kThreads) void unpermute_kernel(const T* __restrict
             ws[s] = slot_weight<WT>(w, p.t * w_stride + min(s0 + s, k - 1));
         }
 #pragma unroll
-        for (int s = 0; s < SLOTS; ++s) v[s] = load_pack_once<T, VEC>(rows + (size_t)max(r[s], 0) * h + (size_t)p.c * VEC);
+        for (int u = 0; u < R; ++u) {
+            const int c = u == 0 || p.c + (u << shift) < hv ? p.c + (u << shift) : p.c;  // past the row: read, not stored
 #pragma unroll
-        for (int s = 0; s < SLOTS; ++s)
+            for (int s = 0; s < SLOTS; ++s) v[u][s] = load_pack_once<T, VEC>(rows + (size_t)max(r[s], 0) * h + (size_t)c * VEC);
+        }
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float x = to_f32<T>(v[s].v[j]);
-                acc[j] = r[s] < 0 ? acc[j] : (WT ? fmaf(ws[s], x, acc[j]) : acc[j] + x);
-            }
+        for (int u = 0; u < R; ++u)
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float x = to_f32<T>(v[u][s].v[j]);
+                    acc[u][j] = r[s] < 0 ? acc[u][j] : (WT ? fmaf(ws[s], x, acc[u][j]) : acc[u][j] + x);
+                }
     }
-    Pack<T, VEC> o;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) o.v[j] = from_f32<T>(acc[j]);
-    store_pack<T, VEC>(y + p.t * h + (size_t)p.c * VEC, o);
+    for (int u = 0; u < R; ++u) {
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o.v[j] = from_f32<T>(acc[u][j]);
+        if (u == 0 || p.c + (u << shift) < hv) store_pack<T, VEC>(y + p.t * h + (size_t)(p.c + (u << shift)) * VEC, o);
+    }
 }
 
 // One CTA per token: dy[t] is read once per batch of slots, every thread keeps one partial dot product per slot, and
@@ -159,22 +182,24 @@ int row_shift(int hv) {
     while (shift < 8 && (1 << shift) < hv) ++shift;
     return shift;
 }
-dim3 grid_for(int n, int hv, int shift) {
+dim3 grid_for(int n, int hv, int shift, int rep) {
     const int tokens = kThreads >> shift;
-    return dim3((unsigned)((n + (size_t)tokens - 1) / tokens), (unsigned)((hv + (1ll << shift) - 1) >> shift));
+    const size_t across = (size_t)rep << shift;
+    return dim3((unsigned)((n + (size_t)tokens - 1) / tokens), (unsigned)((hv + across - 1) / across));
 }
 constexpr int kMaxGridY = 65535;
 
+// bytes = 16 or 4: whether every row of the buffers starts at a multiple of it
 template <typename T>
-bool vectors_ok(int h, const void* a, const void* b, const void* c) {
-    return (size_t)h * sizeof(T) % 16 == 0 &&
-           (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15u) == 0;
+bool vectors_ok(int h, const void* a, const void* b, const void* c, unsigned bytes = 16) {
+    return (size_t)h * sizeof(T) % bytes == 0 &&
+           (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & (bytes - 1)) == 0;
 }
 
 template <typename T, int V>
 int permute_v(const PermuteArgs& a, cudaStream_t stream) {
     const int hv = a.H / V, shift = row_shift(hv);
-    const dim3 grid = grid_for(a.N, hv, shift);
+    const dim3 grid = grid_for(a.N, hv, shift, kPermuteRep<T, V>);
     if (grid.y > kMaxGridY) return XMOE_ERR_LIMIT;
     permute_kernel<T, V><<<grid, kThreads, 0, stream>>>((const T*)a.x, a.topk_row, (T*)a.rows, a.N, hv, a.k, a.idx_stride,
                                                         a.num_rows, shift);
@@ -183,13 +208,15 @@ int permute_v(const PermuteArgs& a, cudaStream_t stream) {
 template <typename T>
 int permute_t(const PermuteArgs& a, cudaStream_t stream) {
     if (vectors_ok<T>(a.H, a.x, a.rows, nullptr)) return permute_v<T, 16 / sizeof(T)>(a, stream);
+    if constexpr (sizeof(T) == 2)
+        if (vectors_ok<T>(a.H, a.x, a.rows, nullptr, 4)) return permute_v<T, 2>(a, stream);
     return permute_v<T, 1>(a, stream);
 }
 
 template <typename T, int V, int WT, int SLOTS>
 int unpermute_s(const PermuteArgs& a, cudaStream_t stream) {
     const int hv = a.H / V, shift = row_shift(hv);
-    const dim3 grid = grid_for(a.N, hv, shift);
+    const dim3 grid = grid_for(a.N, hv, shift, kUnpermuteRep<T, V>);
     if (grid.y > kMaxGridY) return XMOE_ERR_LIMIT;
     unpermute_kernel<T, V, WT, SLOTS><<<grid, kThreads, 0, stream>>>((const T*)a.rows, a.topk_row, a.w, (T*)a.x, a.N, hv, a.k,
                                                                      a.idx_stride, a.w_stride, a.num_rows, shift);
@@ -210,12 +237,16 @@ template <typename T, int WT>
 int unpermute_t(const PermuteArgs& a, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
     if (vectors_ok<T>(a.H, a.x, a.rows, nullptr)) return XMOE_BY_SLOTS(unpermute_s, T, V, WT);
+    if constexpr (sizeof(T) == 2)
+        if (vectors_ok<T>(a.H, a.x, a.rows, nullptr, 4)) return XMOE_BY_SLOTS(unpermute_s, T, 2, WT);
     return XMOE_BY_SLOTS(unpermute_s, T, 1, WT);
 }
 template <typename T, int WT>
 int unpermute_backward_t(const PermuteArgs& a, cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
     if (vectors_ok<T>(a.H, a.x, a.rows, a.drows)) return XMOE_BY_SLOTS(unpermute_backward_s, T, V, WT);
+    if constexpr (sizeof(T) == 2)
+        if (vectors_ok<T>(a.H, a.x, a.rows, a.drows, 4)) return XMOE_BY_SLOTS(unpermute_backward_s, T, 2, WT);
     return XMOE_BY_SLOTS(unpermute_backward_s, T, 1, WT);
 }
 
