@@ -394,8 +394,9 @@ int xmoe_fp8_gemm(const void* x, int32_t ldx, const float* x_scale, int32_t lds,
                   const float* w_scale, int32_t rows, int32_t n, int32_t k, int32_t transpose, void* out, int32_t out_dtype,
                   int32_t ldo, xmoe_stream_t stream);
 /* The same, where the rows [offsets[e], offsets[e] + counts[e]) meet matrix e (device arrays as xmoe_route_pack writes
- * them; a segment must start at a multiple of 16). w: matrix e at byte e * w_mat_stride. Rows outside the segments are
- * left as they were. rows_in_use: an upper bound of the sum of counts that picks the kernel's token tile (0: rows). */
+ * them; a segment must start at a multiple of 16). Where segments overlap, every value of a shared row is the product with
+ * one of their matrices. w: matrix e at byte e * w_mat_stride. Rows outside the segments are left as they were.
+ * rows_in_use: an upper bound of the sum of counts that picks the kernel's token tile (0: rows). */
 int xmoe_fp8_grouped_gemm(const void* x, int32_t ldx, const float* x_scale, int32_t lds, const void* w, int32_t ldw,
                           int64_t w_mat_stride, const float* w_scale, const int32_t* counts, const int32_t* offsets,
                           int32_t mats, int32_t rows, int32_t rows_in_use, int32_t n, int32_t k, int32_t transpose,

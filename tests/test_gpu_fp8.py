@@ -406,6 +406,25 @@ def test_overlapping_segments_beyond_what_can_be_counted():
     assert fp8.status() == 0x700 and bool((out == 7.0).all())
 
 
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("k", [512, 4096])
+def test_overlapping_segments_of_few_tiles(k, transpose):
+    """Eight experts that all claim the same 64 rows make 32 tiles, more than the 12 that segments without overlap could:
+    too few for every SM, so the launch lets clusters share a tile's contraction. Every tile is computed all the same;
+    with one matrix in all eight places every row's product is known."""
+    m, n, e = 64, 128, 8
+    xq, (w, ws) = _operands(m, *((k, n) if transpose else (n, k)), seed=k, transpose=transpose)
+    wq = (torch.empty(e, *w.shape, dtype=w.dtype, device="cuda"), ws.expand(e, *ws.shape).contiguous())
+    wq[0].view(torch.uint8).copy_(w.view(torch.uint8).expand(e, *w.shape))
+    counts = torch.full((e,), m, dtype=torch.int32, device="cuda")
+    offsets = torch.zeros(e + 1, dtype=torch.int32, device="cuda")
+    out = torch.full((m, n), -7.0, device="cuda")
+    y = fp8.grouped_matmul(*xq, *wq, counts, offsets, transpose=transpose, out=out)
+    assert fp8.status() == 0
+    ref, err = _reference(xq, (w, ws), transpose)
+    assert_near(y, ref, 2.0 ** -24 * ref.abs() + err)
+
+
 def test_rows_far_behind_in_a_large_buffer():
     """Offsets beyond 2^31 elements, in codes, outputs and sorted rows."""
     k, r = 8192, 2 ** 18 + 256

@@ -194,8 +194,9 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const int total_tiles = count_tiles(prefix, a.mats, C::kThreads);
-    // a.split > 1: the CTAs of a cluster share one tile, each takes a part of the contraction (a cluster per tile at most)
-    const int split = a.split, rank = split > 1 ? (int)cluster_ctarank() : 0;
+    // a.split > 1: the CTAs of a cluster share one tile, each takes a part of the contraction. The host launches a cluster for
+    // every tile that segments can make which do not overlap; where they overlap and make more, each CTA takes whole tiles.
+    const int split = total_tiles > (int)gridDim.x / a.split ? 1 : a.split, rank = split > 1 ? (int)cluster_ctarank() : 0;
     const int kb_lo = kb_total * rank / split, kb_hi = kb_total * (rank + 1) / split;
     const int units = (int)gridDim.x / split, unit = (int)blockIdx.x / split;
     const int stride = split > 1 ? units : balanced_stride(total_tiles, units);
