@@ -373,7 +373,7 @@ int xmoe_unpermute_backward(const void* dy, const void* rows, const int32_t* top
 int xmoe_fp8_quant(const void* x, int32_t dtype, int32_t rows, int32_t cols, int32_t ldx, const int32_t* topk_row, int32_t k,
                    int32_t idx_stride, int32_t num_rows, void* q, int32_t ldq, float* scale, int32_t lds,
                    xmoe_stream_t stream);
-/* Weights [mats, n, k], contiguous. */
+/* Weights [mats, n, k], contiguous. q [mats, n, ldq]: ldq a multiple of 16, q 16-byte aligned. */
 int xmoe_fp8_quant_weight(const void* w, int32_t dtype, int32_t mats, int32_t n, int32_t k, void* q, int32_t ldq,
                           float* scale, xmoe_stream_t stream);
 /* The gated activation of h = gate | up [rows, 2 * inter], quantised: q [rows, ldq], scale [ceil(inter / 128), lds].

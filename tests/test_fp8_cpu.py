@@ -70,6 +70,12 @@ def test_glu_and_weight_quant_refuse(built_lib):
     assert lib.xmoe_fp8_quant_weight(A, 0, 0, 64, 64, None, 64, None, None) == 0
 
 
+@pytest.mark.parametrize("off", [1, 4, 8])
+def test_weight_quant_refuses_codes_off_16_bytes(built_lib, off):
+    # codes are stored eight at a time, and the products' copies want rows at multiples of 16 bytes
+    assert built_lib.xmoe_fp8_quant_weight(A, 0, 1, 64, 64, A + off, 64, A, None) == SHAPE
+
+
 def test_products_refuse(built_lib):
     lib = built_lib
     names = "x ldx xs lds w ldw wmat ws counts offsets mats rows used n k tr out odt ldo stream".split()

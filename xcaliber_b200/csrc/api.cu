@@ -1274,6 +1274,7 @@ int xmoe_fp8_quant_weight(const void* w, int32_t dtype, int32_t mats, int32_t n,
     if (!is_elem_type(dtype) || n <= 0 || k <= 0 || ldq < k || ldq % 16) return XMOE_ERR_SHAPE;
     if (mats == 0) return XMOE_OK;
     if (!w || !q || !scale) return XMOE_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(q) & 15u) return XMOE_ERR_SHAPE;
     return launch_fp8_quant_weight(w, dtype, mats, n, k, (uint8_t*)q, ldq, scale, (cudaStream_t)stream);
 }
 
