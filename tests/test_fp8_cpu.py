@@ -1,5 +1,7 @@
 """Refusals of the operators around FP8 experts, and the plain forms the GPU tests compare with: no GPU needed."""
 import ctypes as C
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -93,6 +95,22 @@ def test_products_refuse(built_lib):
     assert grouped(rows=0, lds=0) == 0
     assert lib.xmoe_fp8_gemm(A, 120, A, 8, A, 128, A, 8, 256, 128, 0, A, 0, 256, None) == SHAPE
     assert lib.xmoe_fp8_status(None, None) == ARG
+
+
+def test_epilogue_warps_give_up_together():
+    """No lane of an epilogue warp leaves the walk over a tile's blocks by itself, where a shuffle or an aligned tensor-memory
+    read of the whole warp follows; the warp decides behind the walk. (A wait that runs out is not provoked on a GPU; the
+    epilogue sections of the products are read instead.)"""
+    source = (Path(_lib.__file__).parent / "csrc" / "fp8_gemm.cu").read_text()
+    sections = re.findall(r"const int q = warp & 3, part = .*?\n    __syncthreads\(\);", source, re.S)
+    assert len(sections) == 2  # both kernels
+    for text in sections:
+        walk, behind = re.search(r"\n( +)for \(int kb = .*?\n\1\}\n(.*)", text, re.S).group(0, 2)
+        walk = walk[:-len(behind)]
+        voted, own = len(re.findall(r"!mbar_wait_warp\(", walk)), walk.count("ok &= mbar_wait(")
+        assert voted + own == 2 and len(re.findall(r"\bmbar_wait\w*\(", walk)) == 2
+        assert len(re.findall(r"\b(?:break|return|continue|goto)\b", walk)) == voted
+        assert not own or behind.lstrip().startswith("ok = __all_sync(0xffffffffu, ok);")
 
 
 def test_python_refuses_what_it_cannot_do():

@@ -22,7 +22,10 @@
 //
 // Roles: warp 0 TMA producer, warp 1 tensor-memory owner, warps 1 and 3 MMA issuers, warp 2 the tile list, warps 4..
 // epilogue (two per lane quadrant for 128 tokens). Every wait is bounded; a wait that gives up is reported by
-// xmoe_fp8_status.
+// xmoe_fp8_status. An epilogue warp stays whole when some of its lanes give up, so that none is missing in a shuffle or an
+// aligned tensor-memory read: up to 128 tokens the lanes walk on to the end of the tile (their waits return at once then),
+// where the warp decides (a vote at every block costs 1 token 4 %); the pair kernel votes at every block (147 -> 148 us;
+// walking on costs it 3 %).
 #include "cluster.cuh"
 #include "elem.cuh"
 #include "kernels.h"
@@ -84,6 +87,12 @@ __device__ __forceinline__ int count_tiles(const int* prefix, int mats, int thre
 
 __device__ __forceinline__ void st_cluster_f32(uint32_t cluster_addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+
+// The same outcome for all lanes of a warp.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* status,
+                                               uint32_t code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code));
 }
 
 template <int TN>
@@ -291,11 +300,8 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
                 if (((kb - kb_lo) & 31) == 0) ws_lane = kb + lane < kb_hi ? ws[(size_t)(kb + lane) * (TRANS ? w_tiles : 1)] : 0.f;
                 const float sw = __shfl_sync(0xffffffffu, ws_lane, (kb - kb_lo) & 31);
                 const int g = (kb - kb_lo) % C::kGroup;
-                if ((g == 0 && !mbar_wait(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) ||
-                    !mbar_wait(&acc_full[acc], acc_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_ACC)) {
-                    ok = false;
-                    break;
-                }
+                if (g == 0) ok &= mbar_wait(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA);
+                ok &= mbar_wait(&acc_full[acc], acc_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_ACC);
                 tc_fence_after();
                 const float4* xs = reinterpret_cast<const float4*>(scales + (slot * C::kGroup + g) * TN + col0);
                 const uint32_t src = lane_addr + acc * TN;
@@ -329,6 +335,7 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
                     if (++slot == (uint32_t)C::kSlots) { slot = 0; slot_ph ^= 1u; }
                 }
             }
+            ok = __all_sync(0xffffffffu, ok);
             if (split > 1) {
                 // Partial sums to the CTA that stores the column: rank r stores columns [r * TN / split, ..). Once every
                 // CTA of the cluster is past its last MMA (first barrier) the pipeline's stages are free to receive them,
@@ -565,13 +572,13 @@ __global__ __launch_bounds__(kPairThreads, 1) void fp8_gemm_pair_kernel(const __
             for (int kb = 0; kb < kb_total; ++kb) {
                 if ((kb & 31) == 0) ws_lane = kb + lane < kb_total ? ws[(size_t)(kb + lane) * ws_step] : 0.f;
                 const int g = kb % kPairGroup;
-                if (g == 0 && !mbar_wait(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
+                if (g == 0 && !mbar_wait_warp(&sc_full[slot], slot_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_TMA)) {
                     ok = false;
                     break;
                 }
                 const float s = scales[(slot * kPairGroup + g) * 128 + q * 32 + lane] * __shfl_sync(0xffffffffu, ws_lane, kb & 31);
                 const float2 s2 = make_float2(s, s);
-                if (!mbar_wait(&acc_full[acc], acc_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_ACC)) {
+                if (!mbar_wait_warp(&acc_full[acc], acc_ph, abort_flag, &g_fp8_status, XMOE_DEV_TIMEOUT_ACC)) {
                     ok = false;
                     break;
                 }
