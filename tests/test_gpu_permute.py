@@ -8,7 +8,8 @@ import pytest
 import torch
 
 from tests import fp8_plain as P
-from xcaliber_b200 import ops
+from tests import helpers as Hh
+from xcaliber_b200 import ops, synth
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.bfloat16, torch.float16, torch.float32]
@@ -146,6 +147,40 @@ def test_route_pack_gives_every_slot_a_row_of_its_own(n):
         want[t, s] = int(r.offsets[x]) + torch.arange(len(t), dtype=torch.int32)
         assert torch.equal(r.row_token.cpu()[int(r.offsets[x]):int(r.offsets[x]) + len(t)], t.int())
     assert torch.equal(r.topk_row.cpu(), want)
+
+
+def _route_kernels(call):
+    """Names of the route pack's kernels that a call launches."""
+    from torch.profiler import ProfilerActivity, profile
+
+    call()
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        call()
+        torch.cuda.synchronize()
+    names = [e.name for e in p.events()]
+    if not names:
+        pytest.skip("the profiler sees no kernels here")
+    return [n for n in names if "route_scatter_kernel" in n]
+
+
+@pytest.mark.parametrize("n", [9, 300])
+def test_only_routing_of_a_caller_is_checked_for_an_expert_twice(n):
+    """The check costs time: the router's output (of the gated forward too) and a single slot per token go without it."""
+    shape = synth.SHAPES["toy"]
+    w, layer = Hh.build_layer(shape)
+    x, logits = (t.cuda() for t in synth.make_inputs(shape, w, n))
+    gate = w.router_weight.to(torch.bfloat16).cuda()
+    idx, wt = ops.router_topk(logits, shape)
+    unchecked = [lambda: layer.forward_gated(x, gate), lambda: ops.route_pack(idx[:, :1], wt[:, :1], shape.num_experts)]
+    if n > 32:  # smaller batches have a kernel of their own for the whole front
+        unchecked.append(lambda: layer.forward(x, logits))
+    for call in unchecked:
+        names = _route_kernels(call)
+        assert len(names) == 1 and "<false>" in names[0]
+    for call in (lambda: layer.forward_routed(x, idx, wt), lambda: ops.route_pack(idx, wt, shape.num_experts)):
+        names = _route_kernels(call)
+        assert len(names) == 1 and "<true>" in names[0]
 
 
 def test_plan_strides_rows_outside_streams_and_empty_calls():

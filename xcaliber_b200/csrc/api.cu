@@ -400,7 +400,7 @@ int forward_impl(const xmoe_config* cfg, const xmoe_weights* w, const void* x, c
                  const int32_t* ext_idx, const void* ext_w, const float* ext_scale, int n, void* y, void* ws,
                  size_t ws_bytes, cudaStream_t stream, const int32_t* n_valid_dev = nullptr,
                  const xmoe_ep_buffers* ep_ret = nullptr, unsigned long long* row_dst = nullptr,
-                 bool prequantised = false, bool scalars_precleared = false, void* scatter_rows = nullptr) {
+                 bool prequantised = false, bool gated = false, void* scatter_rows = nullptr) {
     int rc = check_cfg(cfg);
     if (prequantised && (!ext_idx || !ext_scale || cfg->top_k + cfg->num_shared_experts != 1)) return XMOE_ERR_ARG;
     if (ep_ret && (!row_dst || !ext_idx || cfg->top_k + cfg->num_shared_experts != 1)) return XMOE_ERR_ARG;
@@ -427,8 +427,9 @@ int forward_impl(const xmoe_config* cfg, const xmoe_weights* w, const void* x, c
     int32_t* offsets = (int32_t*)(b + L.off_offsets);
     const int H = cfg->hidden, I = cfg->inter, E = cfg->num_experts;
 
-    // status words (layer and gate), amax scratch, activation scale
-    if (!scalars_precleared && cudaMemsetAsync(b, 0, kClearedBytes, stream) != cudaSuccess) return XMOE_ERR_CUDA;
+    // status words (layer and gate), amax scratch, activation scale; `gated`: cleared, and the workspace's own routing arrays
+    // written by the router, before this call
+    if (!gated && cudaMemsetAsync(b, 0, kClearedBytes, stream) != cudaSuccess) return XMOE_ERR_CUDA;
     prof_mark(0, stream);
 
     // fork: the amax of x overlaps routing (joined before the quantiser)
@@ -536,7 +537,7 @@ int forward_impl(const xmoe_config* cfg, const xmoe_weights* w, const void* x, c
     }
 
     PackArgs p;
-    p.distinct = ext_idx == nullptr;  // the router names an expert once
+    p.distinct = ext_idx == nullptr || gated;  // the router names an expert once
     p.topk_idx = topk_idx;
     p.topk_w = topk_w;
     p.N = n;
@@ -841,7 +842,7 @@ int xmoe_forward_gated(const xmoe_config* cfg, const xmoe_weights* w, const void
         return rc;
     // the layer takes the routing where it already lies (forward_impl recognises its own arrays)
     return forward_impl(cfg, w, x, nullptr, r.topk_idx, r.topk_w, nullptr, n, y, workspace, workspace_bytes,
-                        (cudaStream_t)stream, nullptr, nullptr, nullptr, false, /*scalars_precleared=*/true);
+                        (cudaStream_t)stream, nullptr, nullptr, nullptr, false, /*gated=*/true);
 }
 
 int xmoe_probe_mma_rate(int32_t kind, int32_t n_mma, double* tflops_out, xmoe_stream_t stream) {

@@ -103,8 +103,8 @@ __global__ __launch_bounds__(256) void route_scatter_kernel(
     if (threadIdx.x == 0) carry = 0;
     __syncthreads();
     const int t_mine = chunk * kPackChunk + threadIdx.x;
-    // CHECK (routing of a caller; a router's has none): whether the token names an expert in several slots: 256 bits of the ids seen so far, and beyond 256 experts, where ids
-    // share a bit, a comparison of all pairs
+    // CHECK (routing of a caller; the router's own and a single slot have none): whether the token names an expert in several
+    // slots: 256 bits of the ids seen so far, and beyond 256 experts, where ids share a bit, a comparison of all pairs
     unsigned long long seen[4] = {0ull, 0ull, 0ull, 0ull};
     bool twice = false;
     if (t_mine < N) {
@@ -322,11 +322,10 @@ int launch_route_pack(const PackArgs& a, cudaStream_t stream) {
     if (chunks > 1)  // a single chunk builds its totals inside the scatter kernel
         route_hist_kernel<<<chunks, 256, 0, stream>>>(a.topk_idx, a.N, a.E, a.topk, a.idx_stride, a.n_shared,
                                                       a.chunk_hist, a.n_valid);
-    auto kernel = a.distinct ? route_scatter_kernel<false> : route_scatter_kernel<true>;
-    kernel<<<chunks, 256, 0, stream>>>(a.topk_idx, (uint16_t*)a.topk_w, a.N, a.E, a.topk,
-                                                     a.idx_stride, a.n_shared, a.chunk_hist, chunks, a.counts,
-                                                     a.offsets, a.topk_off, a.topk_row, a.row_token,
-                                                     (uint16_t*)a.row_weight, a.status, a.n_valid);
+    auto kernel = a.distinct || a.topk <= 1 ? route_scatter_kernel<false> : route_scatter_kernel<true>;
+    kernel<<<chunks, 256, 0, stream>>>(a.topk_idx, (uint16_t*)a.topk_w, a.N, a.E, a.topk, a.idx_stride, a.n_shared,
+                                       a.chunk_hist, chunks, a.counts, a.offsets, a.topk_off, a.topk_row, a.row_token,
+                                       (uint16_t*)a.row_weight, a.status, a.n_valid);
     return cudaGetLastError() == cudaSuccess ? XMOE_OK : XMOE_ERR_CUDA;
 }
 
