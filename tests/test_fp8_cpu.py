@@ -130,6 +130,49 @@ def test_python_refuses_what_it_cannot_do():
         fp8.matmul(x.to(torch.float8_e4m3fn), torch.ones(4, 1), x.to(torch.float8_e4m3fn), torch.ones(1, 1))
 
 
+def calls_into_out(dev):
+    """Every call that writes into tensors of the caller: (name, the tensors, the call)."""
+    n, k, h, r = 4, 2, 64, 128
+    x, rows, plan = torch.zeros(n, h, device=dev), torch.zeros(r, h, device=dev), torch.arange(n * k, dtype=torch.int32).view(n, k).to(dev)
+    w = torch.ones(n, k, device=dev)
+    codes = torch.zeros(n, h, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+    scale = fp8.empty_rows(n, h, dev)[1].zero_()
+    mats = torch.zeros(1, h, h, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+    ws = torch.ones(1, 1, 1, device=dev)
+    counts, offsets = torch.tensor([n], dtype=torch.int32).to(dev), torch.tensor([0, 128], dtype=torch.int32).to(dev)
+    two = torch.zeros(n, 2 * h, device=dev)
+    q = [fp8.empty_rows(m, h, dev) for m in (n, r, n)]
+    y, drows, dh = torch.zeros(n, h, device=dev), torch.zeros(r, h, device=dev), torch.zeros(n, 2 * h, device=dev)
+    a, b = torch.zeros(n, h, device=dev), torch.zeros(n, h, device=dev)
+    return [("permute", [rows], lambda: ops.permute(x, plan, out=rows)),
+            ("unpermute", [y], lambda: ops.unpermute(drows.clone(), plan, w, out=y)),
+            ("unpermute_backward", [drows], lambda: ops.unpermute_backward(x, rows, plan, w, out=drows)),
+            ("quant", list(q[0]), lambda: fp8.quant(x, out=q[0])), ("quant sorted", list(q[1]), lambda: fp8.quant(x, plan, out=q[1])),
+            ("glu_quant", list(q[2]), lambda: fp8.glu_quant(two, out=q[2])),
+            ("glu_backward", [dh], lambda: fp8.glu_backward(x, two, out=dh)),
+            ("matmul", [a], lambda: fp8.matmul(codes, scale, mats[0], ws[0], out=a)),
+            ("grouped_matmul", [b], lambda: fp8.grouped_matmul(codes, scale, mats, ws, counts, offsets, out=b))]
+
+
+def assert_writes_are_seen(dev):
+    for name, outs, call in calls_into_out(dev):
+        before = [t._version for t in outs]
+        call()
+        assert all(t._version > v for t, v in zip(outs, before)), name
+    leaf = torch.zeros(128, 64, device=dev, requires_grad=True)
+    _, (rows,), call = calls_into_out(dev)[0]
+    loss = (leaf * rows).sum()  # keeps rows for the gradient
+    call()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_autograd_sees_writes_into_out():
+    """A tensor of the caller counts as changed by a call that writes into it: a backward pass through a value saved before
+    the write is refused, as after torch's own in-place operations."""
+    assert_writes_are_seen("meta")
+
+
 def test_layout_of_empty_rows():
     codes, scale = fp8.empty_rows(5, 130, "cpu")
     assert codes.shape == (5, 130) and codes.stride() == (144, 1) and codes.dtype == torch.float8_e4m3fn

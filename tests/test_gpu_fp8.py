@@ -447,6 +447,16 @@ def test_rows_far_behind_in_a_large_buffer():
     assert torch.equal(rows, y)
 
 
+def test_autograd_sees_writes_into_out():
+    from tests.test_fp8_cpu import assert_writes_are_seen
+
+    assert_writes_are_seen("cuda")
+    with torch.inference_mode():  # buffers that autograd does not track can be written anywhere
+        x, out = torch.ones(4, 64, device="cuda"), fp8.empty_rows(4, 64, "cuda")
+    fp8.quant(x, out=out)
+    assert_quant(*out, x)
+
+
 # ---- together: the layer ---------------------------------------------------------------------------------------------
 SHAPES = {
     "flat": synth.MoEShape("fp8_flat", 512, 384, 8, 2),

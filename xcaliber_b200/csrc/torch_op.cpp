@@ -175,6 +175,10 @@ int32_t i32(int64_t v, const char* name) {
     return (int32_t)v;
 }
 void check_rc(int rc, const char* what) { TORCH_CHECK(rc == XMOE_OK, what, ": ", xmoe_status_string(rc)); }
+// Marks a tensor of the caller as changed, so that autograd refuses a backward pass through a value saved before the write.
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 xmoe_stream_t stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 // topk_row i32 [N, k], rows of any stride
@@ -203,6 +207,7 @@ void permute_cuda(const at::Tensor& x, const at::Tensor& topk_row, at::Tensor& r
     check_matrix(rows, x, "rows");
     const int32_t ld = check_plan(topk_row, x.size(0), x);
     TORCH_CHECK(rows.scalar_type() == x.scalar_type() && rows.size(1) == x.size(1), "rows must have x's type and width");
+    written(rows);
     if (x.numel() == 0 || rows.numel() == 0 || topk_row.numel() == 0) return;
     c10::cuda::CUDAGuard guard(x.device());
     check_rc(xmoe_permute(x.data_ptr(), topk_row.data_ptr<int32_t>(), i32(x.size(0), "N"), i32(x.size(1), "hidden"),
@@ -218,6 +223,7 @@ void unpermute_cuda(const at::Tensor& rows, const at::Tensor& topk_row, const c1
     const int32_t ld = check_plan(topk_row, y.size(0), rows);
     const SlotWeights w = check_weights(weights, topk_row);
     TORCH_CHECK(rows.scalar_type() == y.scalar_type() && rows.size(1) == y.size(1), "y must have the rows' type and width");
+    written(y);
     if (y.numel() == 0) return;
     c10::cuda::CUDAGuard guard(rows.device());
     check_rc(xmoe_unpermute(rows.data_ptr(), topk_row.data_ptr<int32_t>(), w.p, w.type, w.stride, i32(y.size(0), "N"),
@@ -245,6 +251,8 @@ void unpermute_backward_cuda(const at::Tensor& dy, const at::Tensor& rows, const
     TORCH_CHECK(rows.scalar_type() == dy.scalar_type() && rows.size(1) == dy.size(1), "rows must have dy's type and width");
     TORCH_CHECK(drows.scalar_type() == dy.scalar_type() && drows.sizes() == rows.sizes(), "drows must be like rows");
     TORCH_CHECK(dw.scalar_type() == at::kFloat && dw.sizes() == topk_row.sizes(), "dw must be fp32 [N, k]");
+    written(drows);
+    written(dw);
     if (dw.numel() == 0) return;
     if (dy.size(1) == 0) {
         dw.zero_();
@@ -306,6 +314,8 @@ void fp8_quant_cuda(const at::Tensor& x, const c10::optional<at::Tensor>& topk_r
     const int32_t ldq = check_codes(q, x, "codes");
     const int32_t lds = check_scale_out(scale, q.size(0), x.size(1), x);
     const int32_t ldp = sorted ? check_plan(*topk_row, x.size(0), x) : 0;
+    written(q);
+    written(scale);
     if (x.numel() == 0 || q.numel() == 0 || (sorted && topk_row->numel() == 0)) return;
     c10::cuda::CUDAGuard guard(x.device());
     check_rc(xmoe_fp8_quant(x.data_ptr(), elem_type(x, "x"), i32(x.size(0), "rows"), i32(x.size(1), "cols"),
@@ -324,6 +334,8 @@ void fp8_quant_weight_cuda(const at::Tensor& w, at::Tensor& q, at::Tensor& scale
     TORCH_CHECK(scale.scalar_type() == at::kFloat && scale.dim() == 3 && scale.size(0) == w.size(0) &&
                     scale.size(1) == blocks_of(w.size(1)) && scale.size(2) == blocks_of(w.size(2)),
                 "scale must be fp32 [mats, ceil(n / 128), ceil(k / 128)]");
+    written(q);
+    written(scale);
     if (w.numel() == 0) return;
     c10::cuda::CUDAGuard guard(w.device());
     check_rc(xmoe_fp8_quant_weight(w.data_ptr(), elem_type(w, "w"), i32(w.size(0), "mats"), i32(w.size(1), "n"),
@@ -357,6 +369,8 @@ void glu_fp8_quant_cuda(const at::Tensor& h, int64_t activation, double alpha, d
     const int32_t ldq = check_codes(q, h, "codes");
     const int32_t lds = check_scale_out(scale, q.size(0), q.size(1), h);
     const Segments g = check_segments(counts, offsets, h);
+    written(q);
+    written(scale);
     if (h.numel() == 0) return;
     c10::cuda::CUDAGuard guard(h.device());
     check_rc(xmoe_glu_fp8_quant(h.data_ptr(), elem_type(h, "h"), i32(h.size(0), "rows"), i32(h.size(1) / 2, "inter"),
@@ -375,6 +389,7 @@ void glu_backward_cuda(const at::Tensor& da, const at::Tensor& h, int64_t activa
                 "da must be [rows, inter] of h's type");
     TORCH_CHECK(dh.scalar_type() == h.scalar_type() && dh.sizes() == h.sizes(), "dh must be like h");
     const Segments g = check_segments(counts, offsets, h);
+    written(dh);
     if (h.numel() == 0) return;
     c10::cuda::CUDAGuard guard(h.device());
     check_rc(xmoe_glu_backward(da.data_ptr(), h.data_ptr(), elem_type(h, "h"), i32(h.size(0), "rows"), i32(h.size(1) / 2, "inter"),
@@ -410,6 +425,7 @@ void fp8_product(const at::Tensor& x, const at::Tensor& x_scale, const at::Tenso
         TORCH_CHECK(w.size(0) == 1 || w.stride(0) % 16 == 0, "w's matrices must start at multiples of 16 bytes");
     }
     TORCH_CHECK(rows_in_use >= 0, "rows_in_use must not be negative");
+    written(out);
     if (rows == 0) return;
     c10::cuda::CUDAGuard guard(x.device());
     int64_t lds = scale_ld(x_scale);
@@ -455,19 +471,37 @@ at::Tensor fp8_matmul_new_meta(const at::Tensor& x, const at::Tensor&, const at:
                                at::ScalarType out_dtype) {
     return at::empty({x.size(0), w.size(transpose ? 1 : 0)}, x.options().dtype(out_dtype));
 }
-void permute_meta(const at::Tensor&, const at::Tensor&, at::Tensor&) {}
-void unpermute_meta(const at::Tensor&, const at::Tensor&, const c10::optional<at::Tensor>&, at::Tensor&) {}
+void permute_meta(const at::Tensor&, const at::Tensor&, at::Tensor& rows) { written(rows); }
+void unpermute_meta(const at::Tensor&, const at::Tensor&, const c10::optional<at::Tensor>&, at::Tensor& y) { written(y); }
 void unpermute_backward_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const c10::optional<at::Tensor>&,
-                             at::Tensor&, at::Tensor&) {}
-void fp8_quant_meta(const at::Tensor&, const c10::optional<at::Tensor>&, at::Tensor&, at::Tensor&) {}
-void fp8_quant_weight_meta(const at::Tensor&, at::Tensor&, at::Tensor&) {}
+                             at::Tensor& drows, at::Tensor& dw) {
+    written(drows);
+    written(dw);
+}
+void fp8_quant_meta(const at::Tensor&, const c10::optional<at::Tensor>&, at::Tensor& codes, at::Tensor& scale) {
+    written(codes);
+    written(scale);
+}
+void fp8_quant_weight_meta(const at::Tensor&, at::Tensor& codes, at::Tensor& scale) {
+    written(codes);
+    written(scale);
+}
 void glu_fp8_quant_meta(const at::Tensor&, int64_t, double, double, const c10::optional<at::Tensor>&,
-                        const c10::optional<at::Tensor>&, at::Tensor&, at::Tensor&) {}
+                        const c10::optional<at::Tensor>&, at::Tensor& codes, at::Tensor& scale) {
+    written(codes);
+    written(scale);
+}
 void glu_backward_meta(const at::Tensor&, const at::Tensor&, int64_t, double, double, const c10::optional<at::Tensor>&,
-                       const c10::optional<at::Tensor>&, at::Tensor&) {}
-void fp8_matmul_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, bool, at::Tensor&) {}
+                       const c10::optional<at::Tensor>&, at::Tensor& dh) {
+    written(dh);
+}
+void fp8_matmul_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, bool, at::Tensor& out) {
+    written(out);
+}
 void fp8_grouped_matmul_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
-                             const at::Tensor&, bool, int64_t, at::Tensor&) {}
+                             const at::Tensor&, bool, int64_t, at::Tensor& out) {
+    written(out);
+}
 
 }  // namespace
 
