@@ -173,6 +173,20 @@ def test_autograd_sees_writes_into_out():
     assert_writes_are_seen("meta")
 
 
+def test_out_that_requires_gradients_is_refused():
+    """No call into `out` is recorded for a gradient: a leaf, or a value of an eager graph, is not overwritten in silence."""
+    for k, (name, outs, _) in enumerate(calls_into_out("meta")):
+        for i in range(len(outs)):
+            _, outs, call = calls_into_out("meta")[k]
+            if outs[i].dtype == torch.float8_e4m3fn:
+                continue
+            outs[i].requires_grad_()
+            with pytest.raises(RuntimeError, match="not differentiable"):
+                call()
+            with torch.no_grad():
+                call()
+
+
 def test_layout_of_empty_rows():
     codes, scale = fp8.empty_rows(5, 130, "cpu")
     assert codes.shape == (5, 130) and codes.stride() == (144, 1) and codes.dtype == torch.float8_e4m3fn

@@ -54,6 +54,8 @@ def quant(x: torch.Tensor, topk_row: torch.Tensor | None = None, num_rows: int |
             raise RuntimeError("quant into sorted rows needs num_rows or out")
         else:
             out = _zero_rows(num_rows, x.shape[1], x.device)
+    else:
+        ops._refuse_grad("quant", *out)
     torch_ops.op("fp8_quant")(x, topk_row, out[0], out[1])
     return out
 
@@ -86,6 +88,8 @@ def glu_quant(h: torch.Tensor, activation: str = "silu", alpha: float = 1.702, l
     i = h.shape[1] // 2
     if out is None:
         out = empty_rows(h.shape[0], i, h.device) if counts is None else _zero_rows(h.shape[0], i, h.device)
+    else:
+        ops._refuse_grad("glu_quant", *out)
     torch_ops.op("glu_fp8_quant")(h, _ACT[activation], alpha, limit, counts, offsets, out[0], out[1])
     return out
 
@@ -96,6 +100,8 @@ def glu_backward(da: torch.Tensor, h: torch.Tensor, activation: str = "silu", al
     """The gradient of h from the gradient da [R, I] of the activation (taken as not quantised)."""
     if out is None:
         out = torch.empty_like(h) if counts is None else torch.zeros_like(h)
+    else:
+        ops._refuse_grad("glu_backward", out)
     torch_ops.op("glu_backward")(da, h, _ACT[activation], alpha, limit, counts, offsets, out)
     return out
 
@@ -107,6 +113,7 @@ def matmul(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: tor
     its two scales. Scales of another layout than quant's are laid out anew on every call."""
     if out is None:
         return torch_ops.op("fp8_matmul_new")(x, x_scale, w, w_scale, transpose, out_dtype)
+    ops._refuse_grad("matmul", out)
     torch_ops.op("fp8_matmul")(x, x_scale, w, w_scale, transpose, out)
     return out
 
@@ -119,6 +126,8 @@ def grouped_matmul(rows: torch.Tensor, row_scale: torch.Tensor, w: torch.Tensor,
     rows). `out` keeps the rows outside the segments; without it they are zero."""
     if out is None:
         out = torch.zeros(rows.shape[0], w.shape[-1 if transpose else -2], dtype=out_dtype, device=rows.device)
+    else:
+        ops._refuse_grad("grouped_matmul", out)
     torch_ops.op("fp8_grouped_matmul")(rows, row_scale, w, w_scale, counts, offsets, transpose, rows_in_use, out)
     return out
 

@@ -392,6 +392,12 @@ def route_pack(topk_idx: torch.Tensor, topk_w: torch.Tensor, num_experts: int, n
     return r
 
 
+def _refuse_grad(call: str, *tensors: torch.Tensor) -> None:
+    """A call into tensors of the caller leaves no trace in a graph: those may not require gradients."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{call} into `out` is not differentiable: leave out away, or call it under no_grad")
+
+
 def permute(x: torch.Tensor, topk_row: torch.Tensor, num_rows: int | None = None,
             out: torch.Tensor | None = None) -> torch.Tensor:
     """Tokens to rows sorted by expert: rows[topk_row[t, s]] = x[t]. x [N, H] bf16 / fp16 / fp32, contiguous; topk_row
@@ -403,8 +409,8 @@ def permute(x: torch.Tensor, topk_row: torch.Tensor, num_rows: int | None = None
         if torch.is_grad_enabled() and x.requires_grad:
             return _Permute.apply(x, topk_row, num_rows)
         out = torch.zeros(num_rows, x.shape[-1], dtype=x.dtype, device=x.device)
-    elif torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
-        raise RuntimeError("permute into `out` is not differentiable: leave out away")
+    else:
+        _refuse_grad("permute", x, out)
     torch_ops.op("permute")(x, topk_row, out)
     return out
 
@@ -420,11 +426,12 @@ def unpermute(rows: torch.Tensor, topk_row: torch.Tensor, weights: torch.Tensor 
     bf16 / fp32 [N, k] or None (1). `combine` is the bf16 form without weights that the fused layer ends with.
     Differentiable in rows and weights (without `out`)."""
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
-        if out is not None:
-            raise RuntimeError("unpermute into `out` is not differentiable: leave out away")
-        return _Unpermute.apply(rows, topk_row, weights)
+        if out is None:
+            return _Unpermute.apply(rows, topk_row, weights)
+        _refuse_grad("unpermute", rows, *(() if weights is None else (weights,)))
     if out is None:
         return torch_ops.op("unpermute_new")(rows, topk_row, weights)
+    _refuse_grad("unpermute", out)
     torch_ops.op("unpermute")(rows, topk_row, weights, out)
     return out
 
@@ -434,6 +441,8 @@ def unpermute_backward(dy: torch.Tensor, rows: torch.Tensor, topk_row: torch.Ten
     """The gradients of unpermute: (drows, like rows; dweights fp32 [N, k]). drows[topk_row[t, s]] = weights[t, s] * dy[t],
     dweights[t, s] = <dy[t], rows[topk_row[t, s]]>. `out` receives drows and keeps the rows that no slot names; without it
     they are zero. No row may be named twice."""
+    if out is not None:
+        _refuse_grad("unpermute_backward", out)
     drows = torch.zeros_like(rows) if out is None else out
     dw = torch.empty(topk_row.shape, dtype=torch.float32, device=dy.device)
     torch_ops.op("unpermute_backward")(dy, rows, topk_row, weights, drows, dw)
