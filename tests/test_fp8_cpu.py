@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests import fp8_plain as P
-from xcaliber_b200 import _lib, fp8, ops
+from xcaliber_b200 import _lib, fp8, ops, synth
 
 A = 1 << 20  # an aligned address that no refused call may touch
 ARG, SHAPE, LIMIT = 1, 2, 6
@@ -185,6 +185,28 @@ def test_out_that_requires_gradients_is_refused():
                 call()
             with torch.no_grad():
                 call()
+
+
+def _cpu_layer(**kw):
+    shape = synth.MoEShape("fp8_small", 128, 64, 4, 2, **kw)
+    codes = lambda *d: torch.zeros(*d, dtype=torch.uint8).view(torch.float8_e4m3fn)  # noqa: E731
+    return shape, (codes(4, 128, 128), torch.ones(4, 1, 1), codes(4, 128, 64), torch.ones(4, 1, 1))
+
+
+def test_layer_refuses_tensors_of_other_devices():
+    """Before anything is launched: a kernel would follow the address of another device, or of the host."""
+    shape, weights = _cpu_layer()
+    layer = fp8.Fp8MoE(shape, *weights)
+    x = torch.zeros(4, 128, dtype=torch.bfloat16)
+    logits, idx, w = torch.zeros(4, 4, dtype=torch.bfloat16), torch.zeros(4, 2, dtype=torch.int32), torch.ones(4, 2)
+    for xd in (x, x.to("meta")):
+        with pytest.raises(RuntimeError, match="x must be .* on the device of the weights"):
+            layer.forward(xd, logits)
+        with pytest.raises(RuntimeError, match="x must be .* on the device of the weights"):
+            layer.forward_routed(xd, idx, w)
+    layer.w13 = layer.w13.to("meta")  # stands for a CUDA device
+    with pytest.raises(RuntimeError, match="router_logits must be .* on x's device"):
+        layer._check_logits(x.to("meta"), logits)
 
 
 def test_layout_of_empty_rows():

@@ -208,9 +208,20 @@ class Fp8MoE:
         return grouped_matmul(codes, scale, w, getattr(self, name + "_scale"), r.counts, r.offsets, transpose,
                               r.rows_in_use, out=out)
 
+    def _check_x(self, x):
+        if x.dim() != 2 or x.shape[1] != self.shape.hidden or x.dtype != torch.bfloat16 or not x.is_contiguous():
+            raise RuntimeError("x must be a contiguous bf16 tensor [N, hidden]")
+        if not x.is_cuda or x.device != self.w13.device:
+            raise RuntimeError("x must be a CUDA tensor on the device of the weights")
+
+    def _check_logits(self, x, router_logits):
+        if (router_logits.shape != (x.shape[0], self.shape.num_experts) or router_logits.dtype != torch.bfloat16
+                or router_logits.device != x.device):
+            raise RuntimeError("router_logits must be a bf16 tensor [N, num_experts] on x's device")
+
     def forward(self, x: torch.Tensor, router_logits: torch.Tensor) -> torch.Tensor:
-        if router_logits.shape != (x.shape[0], self.shape.num_experts) or router_logits.dtype != torch.bfloat16:
-            raise RuntimeError("router_logits must be a bf16 tensor [N, num_experts]")
+        self._check_x(x)
+        self._check_logits(x, router_logits)
         if x.shape[0] == 0:
             return torch.empty_like(x)
         with torch.cuda.device(x.device):
@@ -219,8 +230,7 @@ class Fp8MoE:
 
     def forward_routed(self, x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor) -> torch.Tensor:
         """x bf16 [N, H]; topk_idx int32 [N, top_k] (-1: no expert), topk_w bf16 or fp32 [N, top_k]."""
-        if x.dim() != 2 or x.shape[1] != self.shape.hidden or x.dtype != torch.bfloat16 or not x.is_contiguous():
-            raise RuntimeError("x must be a contiguous bf16 tensor [N, hidden]")
+        self._check_x(x)
         if topk_idx.shape != (x.shape[0], self.shape.top_k):
             raise RuntimeError("topk_idx must be [N, top_k]")
         if x.shape[0] == 0:
