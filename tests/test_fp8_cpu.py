@@ -209,6 +209,13 @@ def test_layer_refuses_tensors_of_other_devices():
         layer._check_logits(x.to("meta"), logits)
 
 
+def test_layer_refuses_a_bias_that_is_not_one_per_expert():
+    shape, weights = _cpu_layer(scoring="sigmoid", router_bias=True)
+    for bias in (torch.zeros(3), torch.zeros(8), torch.zeros(4, 1), torch.zeros(())):
+        with pytest.raises(RuntimeError, match="router_bias must be"):
+            fp8.Fp8MoE(shape, *weights, bias)
+
+
 def test_layout_of_empty_rows():
     codes, scale = fp8.empty_rows(5, 130, "cpu")
     assert codes.shape == (5, 130) and codes.stride() == (144, 1) and codes.dtype == torch.float8_e4m3fn

@@ -186,6 +186,8 @@ class Fp8MoE:
             raise RuntimeError("w13 must be [E_tot, 2I, H] and w2 [E_tot, H, I]")
         if shape.act_topk_keep:
             raise RuntimeError("the FP8 layer has no activation top-k")
+        if router_bias is not None and router_bias.shape != (shape.num_experts,):
+            raise RuntimeError("router_bias must be [num_experts]")
         self.shape = shape
         self.w13, self.w13_scale, self.w2, self.w2_scale = w13, w13_scale, w2, w2_scale
         self.router_bias = None if router_bias is None else router_bias.to(w13.device).float().contiguous()
