@@ -345,7 +345,8 @@ int xmoe_forward_gated(const xmoe_config* cfg, const xmoe_weights* w, const void
  * does; xmoe_unpermute alone also takes plans that do). Rows that no slot names are left as they were. Element types:
  * XMOE_BF16 / XMOE_FP16 / XMOE_FP32 for x, y, rows; XMOE_BF16 / XMOE_FP32 for the weights w [n_tokens, w_stride]. Sums in
  * fp32, slot 0 first, rounded once; no atomics. Any hidden size; 16-byte accesses where rows are 16-byte
- * aligned, else 4-byte ones, else (16-bit types of an odd width) one element at a time. */
+ * aligned, else 4-byte ones, else (16-bit types of an odd width) one element at a time. Sizes of these calls and of those
+ * in 8 bits below are refused beyond 2^31 - 1024 (XMOE_ERR_LIMIT). */
 #define XMOE_BF16 0
 #define XMOE_FP16 1
 #define XMOE_FP32 2

@@ -97,6 +97,26 @@ def test_products_refuse(built_lib):
     assert lib.xmoe_fp8_status(None, None) == ARG
 
 
+TOP = 2 ** 31 - 16  # fits 32 bits; a kernel that rounds it up to its next step does not
+
+
+def test_sizes_at_the_end_of_32_bits_are_refused(built_lib):
+    """Kernels step through rows and columns in 32 bits, past the last by up to a block or a CTA's share."""
+    lib = built_lib
+    assert lib.xmoe_permute(A, A, 4, TOP, 2, 2, 128, 2, A, None) == LIMIT
+    assert lib.xmoe_unpermute_backward(A, 2 * A, A, None, 0, 0, 1, TOP, 2, 2, 1, 2, 4 * A, A, None) == LIMIT
+    assert lib.xmoe_unpermute(A, A, None, 0, 0, 1, 64, TOP, TOP, 128, 0, A, None) == LIMIT
+    assert lib.xmoe_fp8_quant(A, 0, TOP, 1, 1, None, 0, 0, 0, A, 16, A, TOP, None) == LIMIT
+    assert lib.xmoe_fp8_quant(A, 0, 1, TOP, TOP, None, 0, 0, 0, A, TOP, A, 4, None) == LIMIT
+    assert lib.xmoe_fp8_quant(A, 0, 1, 64, 64, A, TOP, TOP, 128, A, 64, A, 128, None) == LIMIT
+    assert lib.xmoe_fp8_quant_weight(A, 0, 1, TOP, 1, A, 16, A, None) == LIMIT
+    assert lib.xmoe_fp8_quant_weight(A, 0, 1, 1, TOP, A, TOP, A, None) == LIMIT
+    assert lib.xmoe_glu_fp8_quant(A, 0, TOP, 1, 0, 1.0, 1.0, None, None, 0, A, 16, A, TOP, None) == LIMIT
+    assert lib.xmoe_glu_backward(A, A, 0, TOP, 1, 0, 1.0, 1.0, None, None, 0, 2 * A, None) == LIMIT
+    for rows, n, k in ((TOP, 1, 16), (1, TOP, 16), (1, 16, TOP)):
+        assert lib.xmoe_fp8_gemm(A, max(k, 16), A, max(rows, 4), A, max(k, 16), A, rows, n, k, 0, A, 0, n, None) == LIMIT
+
+
 def test_epilogue_warps_give_up_together():
     """No lane of an epilogue warp leaves the walk over a tile's blocks by itself, where a shuffle or an aligned tensor-memory
     read of the whole warp follows; the warp decides behind the walk. (A wait that runs out is not provoked on a GPU; the

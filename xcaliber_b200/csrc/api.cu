@@ -645,12 +645,19 @@ int forward_impl(const xmoe_config* cfg, const xmoe_weights* w, const void* x, c
 // ---- operators around FP8 experts ---------------------------------------------------------------------------
 bool is_elem_type(int dtype) { return dtype == XMOE_BF16 || dtype == XMOE_FP16 || dtype == XMOE_FP32; }
 
+// Kernels step through rows, columns and slots in 32 bits and pass the last by up to a block or a CTA's share.
+bool beyond_steps(int a, int b = 0, int c = 0) {
+    constexpr int kMost = 0x7fffffff - 1023;
+    return a > kMost || b > kMost || c > kMost;
+}
+
 // Arguments that the three permutations share. Returns XMOE_OK with *empty set when there is nothing to do.
 int check_permute(const PermuteArgs& a, bool* empty) {
     *empty = false;
     if (a.N < 0 || a.k < 0 || a.num_rows < 0) return XMOE_ERR_ARG;
     if (!is_elem_type(a.dtype) || (a.w && a.w_dtype != XMOE_BF16 && a.w_dtype != XMOE_FP32)) return XMOE_ERR_SHAPE;
     if (a.H <= 0 || a.idx_stride < a.k || (a.w && a.w_stride < a.k)) return XMOE_ERR_SHAPE;
+    if (beyond_steps(a.H, a.k)) return XMOE_ERR_LIMIT;
     *empty = a.N == 0;
     if (*empty) return XMOE_OK;
     if (!a.x || (!a.topk_row && a.k) || (!a.rows && a.num_rows && a.k)) return XMOE_ERR_ARG;
@@ -669,7 +676,7 @@ int run_fp8_gemm(const void* x, int ldx, const float* x_scale, int lds, const vo
                  int n, int k, bool transpose, void* out, int out_dtype, int ldo, cudaStream_t stream) {
     if (rows < 0 || rows_in_use < 0) return XMOE_ERR_ARG;
     if (n <= 0 || k <= 0 || mats <= 0 || !is_elem_type(out_dtype)) return XMOE_ERR_SHAPE;
-    if (mats > 1032) return XMOE_ERR_LIMIT;
+    if (mats > 1032 || beyond_steps(rows, n, k)) return XMOE_ERR_LIMIT;
     const int contraction = transpose ? n : k, features = transpose ? k : n;
     if (ldx < contraction || ldx % 16 || ldw < k || ldw % 16 || lds < rows || lds % 4 || ldo < features) return XMOE_ERR_SHAPE;
     if (mats > 1 && (w_mat_stride < (int64_t)ldw * (n - 1) + k || w_mat_stride % 16)) return XMOE_ERR_SHAPE;
@@ -1248,6 +1255,7 @@ int xmoe_fp8_quant(const void* x, int32_t dtype, int32_t rows, int32_t cols, int
     if (rows < 0 || (topk_row && (k < 0 || num_rows < 0))) return XMOE_ERR_ARG;
     if (!is_elem_type(dtype) || cols <= 0 || ldx < cols || ldq < cols || ldq % 16 || lds % 4) return XMOE_ERR_SHAPE;
     if (topk_row ? (idx_stride < k || lds < num_rows) : lds < rows) return XMOE_ERR_SHAPE;
+    if (beyond_steps(rows, cols, topk_row ? k : 0)) return XMOE_ERR_LIMIT;
     if (rows == 0 || (topk_row && (k == 0 || num_rows == 0))) return XMOE_OK;
     if (!x || !q || !scale) return XMOE_ERR_ARG;
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(scale)) & 15u) return XMOE_ERR_SHAPE;
@@ -1273,6 +1281,7 @@ int xmoe_fp8_quant_weight(const void* w, int32_t dtype, int32_t mats, int32_t n,
                           float* scale, xmoe_stream_t stream) {
     if (mats < 0) return XMOE_ERR_ARG;
     if (!is_elem_type(dtype) || n <= 0 || k <= 0 || ldq < k || ldq % 16) return XMOE_ERR_SHAPE;
+    if (beyond_steps(n, k)) return XMOE_ERR_LIMIT;
     if (mats == 0) return XMOE_OK;
     if (!w || !q || !scale) return XMOE_ERR_ARG;
     if (reinterpret_cast<uintptr_t>(q) & 15u) return XMOE_ERR_SHAPE;
@@ -1286,7 +1295,7 @@ int xmoe_glu_fp8_quant(const void* h, int32_t dtype, int32_t rows, int32_t inter
     if (!is_elem_type(dtype) || inter <= 0 || activation < 0 || activation > 2 || ldq < inter || ldq % 16 || lds < rows || lds % 4)
         return XMOE_ERR_SHAPE;
     if (inter > 0x3fffffff || (counts && (!offsets || mats <= 0))) return XMOE_ERR_ARG;
-    if (counts && mats > 1032) return XMOE_ERR_LIMIT;
+    if ((counts && mats > 1032) || beyond_steps(rows)) return XMOE_ERR_LIMIT;
     if (rows == 0) return XMOE_OK;
     if (!h || !q || !scale) return XMOE_ERR_ARG;
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(scale)) & 15u) return XMOE_ERR_SHAPE;
@@ -1316,7 +1325,7 @@ int xmoe_glu_backward(const void* da, const void* h, int32_t dtype, int32_t rows
     if (rows < 0) return XMOE_ERR_ARG;
     if (!is_elem_type(dtype) || inter <= 0 || activation < 0 || activation > 2) return XMOE_ERR_SHAPE;
     if (inter > 0x3fffffff || (counts && (!offsets || mats <= 0))) return XMOE_ERR_ARG;
-    if (counts && mats > 1032) return XMOE_ERR_LIMIT;
+    if ((counts && mats > 1032) || beyond_steps(rows)) return XMOE_ERR_LIMIT;
     if (rows == 0) return XMOE_OK;
     if (!da || !h || !dh || dh == h) return XMOE_ERR_ARG;
     Fp8QuantArgs a;
