@@ -117,6 +117,13 @@ def test_sizes_at_the_end_of_32_bits_are_refused(built_lib):
         assert lib.xmoe_fp8_gemm(A, max(k, 16), A, max(rows, 4), A, max(k, 16), A, rows, n, k, 0, A, 0, n, None) == LIMIT
 
 
+@pytest.mark.parametrize("n,e,k,shared,rc", [(2 ** 26, 8, 32, 0, LIMIT), (2 ** 31 - 1, 8, 1, 0, LIMIT), (2 ** 27 - 1, 512, 16, 0, LIMIT),
+                                             (4, -1, 2, 2, SHAPE), (4, 8, 2, -1, SHAPE), (4, 8, -1, 2, SHAPE)])
+def test_route_pack_refuses(built_lib, n, e, k, shared, rc):
+    """Row numbers are 32-bit, padding of the experts' segments included."""
+    assert built_lib.xmoe_route_pack(A, A, n, e, k, max(k + shared, 8), shared, A, A, A, A, A, A, A, A, None) == rc
+
+
 def test_epilogue_warps_give_up_together():
     """No lane of an epilogue warp leaves the walk over a tile's blocks by itself, where a shuffle or an aligned tensor-memory
     read of the whole warp follows; the warp decides behind the walk. (A wait that runs out is not provoked on a GPU; the

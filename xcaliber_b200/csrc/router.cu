@@ -317,7 +317,12 @@ int route_pack_chunks(int N) { return (N + kPackChunk - 1) / kPackChunk; }
 
 int launch_route_pack(const PackArgs& a, cudaStream_t stream) {
     if (a.N <= 0) return XMOE_OK;
-    if (a.E + a.n_shared > kMaxEtot || a.topk + a.n_shared > 32) return XMOE_ERR_SHAPE;
+    if (a.E < 0 || a.n_shared < 0 || a.topk < 0 || a.E > kMaxEtot || a.n_shared > 32 || a.topk > 32 ||
+        a.E + a.n_shared > kMaxEtot || a.topk + a.n_shared > 32)
+        return XMOE_ERR_SHAPE;
+    // row numbers have 31 bits; every expert's segment is padded to a multiple of 128
+    const long long slots = (long long)a.N * max(a.topk + a.n_shared, 1);
+    if (slots + 127ll * (a.E + a.n_shared) > 0x7fffffffll) return XMOE_ERR_LIMIT;
     const int chunks = route_pack_chunks(a.N);
     if (chunks > 1)  // a single chunk builds its totals inside the scatter kernel
         route_hist_kernel<<<chunks, 256, 0, stream>>>(a.topk_idx, a.N, a.E, a.topk, a.idx_stride, a.n_shared,
