@@ -557,6 +557,22 @@ def test_layer_with_an_expert_twice_and_with_nothing():
     assert not y.any() and not gx.any() and not gw.any() and fp8.status() == 0
 
 
+@pytest.mark.parametrize("name", list(SHAPES))
+def test_layer_without_tokens_stays_in_the_graph(name):
+    """A rank whose share of a batch is empty takes its backward step like the others."""
+    shape = SHAPES[name]
+    layer = _layer(shape)
+    x = torch.empty(0, shape.hidden, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    w = torch.empty(0, shape.top_k, device="cuda", requires_grad=True)
+    idx = torch.empty(0, shape.top_k, dtype=torch.int32, device="cuda")
+    y = layer.forward_routed(x, idx, w)
+    assert y.shape == (0, shape.hidden) and y.dtype == torch.bfloat16
+    gx, gw = torch.autograd.grad(y.sum(), (x, w))
+    assert gx.shape == x.shape and gw.shape == w.shape and gw.dtype == w.dtype
+    y = layer.forward(x, torch.empty(0, shape.num_experts, device="cuda", dtype=torch.bfloat16))
+    assert torch.autograd.grad(y.sum(), x)[0].shape == x.shape and fp8.status() == 0
+
+
 def test_products_in_flight_together():
     """Large and small products (CTA pairs, clusters that share a tile, plain CTAs) on three streams at once."""
     jobs = [_operands(700, 2048, 1024, seed=1), _operands(3, 512, 4096, seed=2), _operands(40, 3000, 512, seed=3)]

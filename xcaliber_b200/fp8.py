@@ -224,8 +224,9 @@ class Fp8MoE:
     def forward(self, x: torch.Tensor, router_logits: torch.Tensor) -> torch.Tensor:
         self._check_x(x)
         self._check_logits(x, router_logits)
-        if x.shape[0] == 0:
-            return torch.empty_like(x)
+        if x.shape[0] == 0:  # nothing to route
+            idx, w = (torch.empty(0, self.shape.top_k, dtype=t, device=x.device) for t in (torch.int32, torch.bfloat16))
+            return self.forward_routed(x, idx, w)
         with torch.cuda.device(x.device):
             idx, w = ops.router_topk(router_logits.contiguous(), self.shape, self)
         return self.forward_routed(x, idx, w)
@@ -235,8 +236,6 @@ class Fp8MoE:
         self._check_x(x)
         if topk_idx.shape != (x.shape[0], self.shape.top_k):
             raise RuntimeError("topk_idx must be [N, top_k]")
-        if x.shape[0] == 0:
-            return torch.empty_like(x)
         shared = self.shape.num_shared_experts
         r = ops.route_pack(topk_idx, topk_w.detach().to(torch.bfloat16), self.shape.num_experts, shared)
         w = topk_w
