@@ -198,6 +198,30 @@ def test_glu_quant_and_gradient(n, e, k, inter, name, dtype):
     assert_near(dh[live], ref, rel * ref.abs() + floor + err * size)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("name", ["silu", "swiglu_clamp", "gelu_tanh"])
+def test_glu_gradient_of_huge_gates(name, dtype):
+    """Gates up to the type's largest: the sigmoid is 0 or 1 there (below e^-100 or above 1 - e^-100), its slope 0, and the
+    gradients are da u or 0 and da g or 0, one rounding each of the two products and one to the type."""
+    most = torch.finfo(dtype).max
+    g = torch.tensor([1e3, 1e6, 3e12, 1.5e13, 1e15, 1e19, 1e25, 1e38, most], device="cuda")
+    g = torch.cat([g, -g]).to(dtype)
+    i = g.numel()
+    u, da = torch.full((i,), 1.5, device="cuda", dtype=dtype), torch.full((i,), 0.125, device="cuda", dtype=dtype)
+    dh = fp8.glu_backward(da[None], torch.cat([g, u])[None], name)[0].double()
+    up = (g > 0).double()
+    want_g = 0.125 * 1.5 * up
+    want_u = 0.125 * g.double() * up
+    if name == "swiglu_clamp":  # gates above the limit have no gradient and count as the limit, where the sigmoid is not yet 1
+        want_g, want_u = 0 * up, 0.125 * 7 * torch.sigmoid(torch.tensor(1.702 * 7.0, dtype=torch.float64)) * up
+    rel = half_step(dtype)[0] + (2 + 8 + 4 * 12) * 2.0 ** -23 * (name == "swiglu_clamp") + 2.0 ** -23
+    assert_near(dh[:i], want_g, rel * want_g.abs())
+    assert_near(dh[i:], want_u, rel * want_u.abs())
+    nan = torch.cat([torch.full((8,), float("nan"), device="cuda", dtype=dtype), torch.ones(8, device="cuda", dtype=dtype)])[None]
+    dn = fp8.glu_backward(torch.ones(1, 8, device="cuda", dtype=dtype), nan, name)
+    assert bool(dn[0, 8:].isnan().all()) and (name == "swiglu_clamp" or bool(dn[0, :8].isnan().all()))
+
+
 def test_glu_keeps_nan_and_saturates():
     h = torch.zeros(1, 256, device="cuda")
     h[0, 5], h[0, 133] = float("nan"), 1.0

@@ -265,17 +265,20 @@ __device__ __forceinline__ float glu_value(float g, float u, float alpha, float 
     if (ACT == 2) return g * sigmoid(2.f * kGeluC * (g + kGeluA * g * g * g)) * u;
     return g * sigmoid(g) * u;
 }
+// The derivative has a factor z' (1 - s) or z (1 - s) that goes to zero as z grows; z is kept inside where s is still neither
+// 0 nor 1 or has just become it, so that the factor is that zero instead of infinity times zero (NaN) for huge gates.
 template <int ACT>
 __device__ __forceinline__ void glu_gradient(float g, float u, float da, float alpha, float limit, float& dg, float& du) {
     if (ACT == 1) {
         const bool in_g = g <= limit, in_u = fabsf(u) <= limit;
         const float gc = g > limit ? limit : g, uc = u > limit ? limit : (u < -limit ? -limit : u);
-        const float s = sigmoid(alpha * gc);
-        dg = in_g ? da * (uc + 1.f) * s * (1.f + alpha * gc * (1.f - s)) : 0.f;
+        const float z = alpha * gc, s = sigmoid(z);
+        dg = in_g ? da * (uc + 1.f) * s * (1.f + fminf(fmaxf(z, -256.f), 256.f) * (1.f - s)) : 0.f;
         du = in_u ? da * gc * s : 0.f;
     } else if (ACT == 2) {
         const float s = sigmoid(2.f * kGeluC * (g + kGeluA * g * g * g));
-        dg = da * u * s * (1.f + 2.f * kGeluC * g * (1.f + 3.f * kGeluA * g * g) * (1.f - s));
+        const float gc = fminf(fmaxf(g, -64.f), 64.f);
+        dg = da * u * s * (1.f + 2.f * kGeluC * gc * (1.f + 3.f * kGeluA * gc * gc) * (1.f - s));
         du = da * g * s;
     } else {
         const float s = sigmoid(g);
