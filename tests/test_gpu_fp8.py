@@ -471,6 +471,38 @@ def test_rows_far_behind_in_a_large_buffer():
     assert torch.equal(rows, y)
 
 
+def _registered_calls():
+    row, counts, offsets, r = P.plan(12, 4, 2, seed=1)
+    plan, c, o, dev, h = row.cuda(), counts.cuda(), offsets.cuda(), "cuda", 256
+    x, rows, w = torch.randn(12, h, device=dev), torch.randn(r, h, device=dev), torch.rand(12, 2, device=dev)
+    xq, wm = fp8.quant(x, plan, r), torch.randn(4, 128, h, device=dev)
+    wq = fp8.quant_weight(wm)
+    z = lambda *d: torch.zeros(*d, device=dev)  # noqa: E731
+    codes = lambda *d: torch.zeros(*d, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)  # noqa: E731
+    return {"permute": (x, plan, z(r, h)), "unpermute": (rows, plan, w, z(12, h)), "unpermute_new": (rows, plan, w),
+            "unpermute_backward": (x, rows, plan, w, z(r, h), z(12, 2)),
+            "glu_backward": (rows[:, :128].contiguous(), rows, 0, 1.702, 7.0, c, o, z(r, h)),
+            "fp8_quant": (x, plan, codes(r, h), fp8.empty_rows(r, h, dev)[1].zero_()),
+            "fp8_quant_weight": (wm, codes(4, 128, h), z(4, 1, 2)),
+            "glu_fp8_quant": (rows, 0, 1.702, 7.0, c, o, codes(r, h // 2), fp8.empty_rows(r, h // 2, dev)[1].zero_()),
+            "fp8_matmul": (*xq, wq[0][0], wq[1][0], False, z(r, 128)),
+            "fp8_matmul_new": (*xq, wq[0][0], wq[1][0], False, torch.bfloat16),
+            "fp8_grouped_matmul": (*xq, *wq, c, o, False, 0, z(r, 128))}
+
+
+@pytest.mark.parametrize("name", ["permute", "unpermute", "unpermute_new", "unpermute_backward", "glu_backward", "fp8_quant",
+                                  "fp8_quant_weight", "glu_fp8_quant", "fp8_matmul", "fp8_matmul_new", "fp8_grouped_matmul"])
+def test_registered_ops_hold_to_their_schemas(name):
+    """What torch asks of a registered op: it changes what its schema says and nothing else, its fake form has the real
+    one's results, and it traces. (The schema check multiplies its inputs, which torch cannot do for 8-bit floats.)"""
+    args = _registered_calls()[name]
+    op = getattr(torch.ops.xmoe_b200, name).default
+    tests = ["test_autograd_registration", "test_faketensor", "test_aot_dispatch_dynamic"]
+    if not any(isinstance(a, torch.Tensor) and a.dtype == torch.float8_e4m3fn for a in args):
+        tests.append("test_schema")
+    torch.library.opcheck(op, args, test_utils=tests)
+
+
 def test_autograd_sees_writes_into_out():
     from tests.test_fp8_cpu import assert_writes_are_seen
 
