@@ -688,7 +688,8 @@ int run_fp8_gemm(const void* x, int ldx, const float* x_scale, int lds, const vo
     int tile = fp8_token_tile((size_t)(rows_in_use && rows_in_use < rows ? rows_in_use : rows), (size_t)mats);
     // one matrix, few tiles and a long contraction: where 128-token tiles leave two CTAs for each, sharing a tile's
     // contraction beats CTA pairs (200 tokens, weight 4096 x 7168: 28 against 34 us, 2880 x 5760: 25 against 29; a short
-    // contraction does not pay for the exchange, 400 tokens, 1536 x 2048: 17 against 15)
+    // contraction does not pay for the exchange, 400 tokens, 1536 x 2048: 17 against 15; nothing between 2048 and 5760
+    // was measured, 4096 is a guess)
     if (tile == 256 && !counts && contraction >= 4096 &&
         (size_t)((rows + 127) / 128) * (size_t)((features + 127) / 128) * 2 <= (size_t)num_sms())
         tile = 128;

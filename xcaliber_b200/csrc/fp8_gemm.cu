@@ -13,12 +13,16 @@
 // side and the tokens its N side. The weight's scale is one number per tile and block, ragged token counts only narrow the
 // MMA, and a decode batch of a few tokens costs a narrow MMA instead of a mostly empty one. Such calls are bound by the
 // weight's bytes (128 experts of 1536 x 2048, 16 tokens, 181 MB from HBM: 35 us = 5.2 TB/s) or, with few tiles, by latency
-// (4096 x 7168, 1 token: 8.4 us on the device, 15 blocks of ~400 cycles behind launch, set-up and exchange).
-// Larger ones run on CTA pairs with the roles exchanged (fp8_gemm_pair_kernel, below): 4096 x 4096 x 7168 in 147 us, 1.63
-// PFLOP/s.
+// (4096 x 7168, 1 token: 9.4 us on the device, 14 blocks of ~400 cycles behind launch, set-up and exchange). In between
+// (4096 x 7168: 64 tokens 17 us, 100 20, 200 31) neither bytes nor arithmetic bound it: a CTA has 14 to 28 blocks, and
+// every value added fetches its own token scale from shared memory.
+// Larger ones run on CTA pairs with the roles exchanged (fp8_gemm_pair_kernel, below): 4096 x 4096 x 7168 in 134 us, 1.79
+// PFLOP/s, when the GPU was idle before, and 148 us, 1.63 PFLOP/s, back to back, where the power cap holds the clock at
+// 1680 MHz.
 //
 // TRANS reads the same 128 x 128 weight box from shared memory with the operand's transpose bit (features contiguous), so
-// one copy of the weight serves both directions at the same speed (131 against 132 us for that product).
+// one copy of the weight serves both directions, at nearly the same speed (the same sums from a transposed weight: 141
+// against 134 us, 152 against 147 back to back).
 //
 // Roles: warp 0 TMA producer, warp 1 tensor-memory owner, warps 1 and 3 MMA issuers, warp 2 the tile list, warps 4..
 // epilogue (two per lane quadrant for 128 tokens). Every wait is bounded; a wait that gives up is reported by
@@ -393,12 +397,14 @@ __global__ __launch_bounds__(Cfg<TN>::kThreads, 1) void fp8_gemm_kernel(const __
 // Each CTA of the pair stages its 128 tokens and 128 of the 256 features: 32 KB per 128 columns of K instead of 48, which one
 // CTA alone would take in and read (128 x 256 tiles on single CTAs: 165 us).
 //
-// What bounds it: a block takes ~1000 cycles where its MMAs take 512 (ncu: tensor pipe active 51 %). Tensor memory holds two
-// accumulators, and an accumulator comes round again only after the MMAs (512), a wake-up of the epilogue, its reads and
-// additions (430) and a wake-up of the issuing thread across the pair. Halving the accumulators (N 128) frees them earlier
-// but doubles the reads of the token operand: 158 to 174 us. Global loads of the scales inside the loop cost 125 cycles a
-// block, hence the ring in shared memory and the lane registers. One product of the same size without block scales (one
-// accumulator for the whole contraction, library call): 8192 x 4096 x 7168 in 165 us against 240 here.
+// What bounds it: a block takes ~1000 cycles where its MMAs take 512 (ncu: tensor pipe active 51 %, DRAM 6 %). An
+// accumulator comes round again only after its MMAs, a wake-up of the epilogue, its reads and additions (430) and a wake-up
+// of the issuing thread across the pair: 1000 cycles is about that round trip, as if there were one accumulator. There are
+// two, which in turn should take little over half of it, so what holds a block back is not established. Halving the
+// accumulators (N 128) frees them earlier but doubles the reads of the token operand: 158 to 174 us. Global loads of the
+// scales inside the loop cost 125 cycles a block, hence the ring in shared memory and the lane registers. One product of
+// the same size without block scales (one accumulator for the whole contraction, library call): 8192 x 4096 x 7168 in 165
+// us against 242 here.
 constexpr int kPairStages = 6, kPairThreads = 384, kPairEpiWarps = 8;
 constexpr int kPairStageBytes = 2 * kBoxBytes;
 constexpr int kPairGroup = 2, kPairSlots = 4;  // token scales: as in Cfg

@@ -9,10 +9,15 @@
 // shuffles for the maximum, two 8-byte stores. Scales are stored block-major, [ceil(cols / 128), lds], the order in which the product
 // reads them: the scales of consecutive rows for one block are contiguous.
 //
-// Bound by instructions rather than bytes where the input has 16 bits: about 15 per value of which 8 are on the half-rate
-// integer pipe (unpacking, maxima, conversions), and ties of two codes, which bf16 values with a bf16 maximum meet in one
-// block of 14, cost a branch. Measured: fp32 8192 x 4096 31 us = 5.5 TB/s, bf16 8192 x 7168 55 us = 3.2 TB/s, gated
-// activation of 16384 rows of 2 x 2880 60 to 71 us = 3.4 to 4.0 TB/s, its gradient 100 to 119 us = 4.0 to 4.7 TB/s.
+// Measured: fp32 8192 x 4096 31 us = 5.4 TB/s; bf16 8192 x 7168 55 us = 3.2 TB/s, fp16 45 us = 3.9 TB/s; gated activation
+// of 16384 rows of 2 x 2880 58 (silu) to 69 us (clamped) = 3.4 to 4.1 TB/s, its gradient 98 to 119 us = 4.0 to 4.8 TB/s;
+// weights 32 x 4096 x 7168 1.74 ms = 1.6 TB/s (load time). Rows that are not 16-byte aligned are read element by element:
+// 49024 rows of 2050 bf16 in 99 us against 92 for 2048 aligned ones.
+// fp32 rows are bound by bytes. With 16-bit inputs neither bytes nor instructions are at their limit: about 15 instructions
+// per value (8 of them on the half-rate integer pipe) are 24 of the 55 us, the bytes 27; a warp loads, waits, computes and
+// stores in turn with no load of its next step in flight, so latency is the likely rest. Ties of two codes cost a branch,
+// which bf16 values with a bf16 maximum meet in one block of 14. The gated activation and its gradient are alike: issue 63
+// to 67 %, DRAM 32 to 44 %.
 #include "elem.cuh"
 #include "kernels.h"
 #include "tile_sched.cuh"

@@ -10,7 +10,9 @@
 // All three move bytes and do next to no arithmetic: each token's data is read once and all its slots are served from
 // registers, so HBM traffic is the floor (one read of every input, one write of every output). Measured, 8191 tokens, 8
 // slots, 2048 bf16: unpermute 47.5 us = 6.4 TB/s, its gradient 95 us = 6.0 TB/s; 4095 tokens, 4 slots, 2880 fp16: permute
-// 21 us = 5.4 TB/s and its gradient 21 us = 5.6 TB/s.
+// 21 us = 5.4 TB/s and its gradient 21 us = 5.6 TB/s. Rows of 16-bit values that are not 16-byte aligned take narrower
+// accesses (4096 tokens, 8 slots; permute, unpermute, its gradient): width 2048 26, 25, 48 us; 2050, 4 bytes each, 41, 41,
+// 72; 2049, 2 bytes each, 50, 92, 214.
 #include "elem.cuh"
 #include "kernels.h"
 

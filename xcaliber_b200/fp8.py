@@ -5,6 +5,9 @@ row and 128 columns; a value is code * scale. Activation scales are kept block-m
 strides (1, ld)), the order in which the product reads them; codes' rows start at multiples of 16 bytes. `quant`,
 `glu_quant` and `quant_weight` return both in that layout.
 
+The functions have no gradient of their own, whatever their inputs require: gradients come from `Fp8MoE.forward_routed`, or by
+hand from `glu_backward` and the products with transpose=True.
+
 All compute is in libxmoe_b200.so (through the registered ops of torch_ops.py); a missing library or a failed call raises.
 """
 from __future__ import annotations
@@ -122,8 +125,9 @@ def grouped_matmul(rows: torch.Tensor, row_scale: torch.Tensor, w: torch.Tensor,
                    counts: torch.Tensor, offsets: torch.Tensor, transpose: bool = False, rows_in_use: int = 0,
                    out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """matmul, where rows [offsets[e], offsets[e] + counts[e]) meet matrix e of w [E, N, K]. Segments start at multiples
-    of 16 (ops.route_pack: of 128). rows_in_use: an upper bound of the sum of counts, it picks the kernel's tile (0: all
-    rows). `out` keeps the rows outside the segments; without it they are zero."""
+    of 16 (ops.route_pack: of 128). rows_in_use: an upper bound of the sum of counts, it picks the kernel's tile. Pass it
+    for small batches: 0 stands for all rows, the padding between segments too, and a decode batch then runs in tiles many
+    times its size. `out` keeps the rows outside the segments; without it they are zero."""
     if out is None:
         out = torch.zeros(rows.shape[0], w.shape[-1 if transpose else -2], dtype=out_dtype, device=rows.device)
     else:
@@ -232,7 +236,8 @@ class Fp8MoE:
         return self.forward_routed(x, idx, w)
 
     def forward_routed(self, x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tensor) -> torch.Tensor:
-        """x bf16 [N, H]; topk_idx int32 [N, top_k] (-1: no expert), topk_w bf16 or fp32 [N, top_k]."""
+        """x bf16 [N, H]; topk_idx int32 [N, top_k] (-1: no expert, as is any other id outside the routed experts), topk_w
+        bf16 or fp32 [N, top_k]."""
         self._check_x(x)
         if topk_idx.shape != (x.shape[0], self.shape.top_k):
             raise RuntimeError("topk_idx must be [N, top_k]")

@@ -424,7 +424,8 @@ def unpermute(rows: torch.Tensor, topk_row: torch.Tensor, weights: torch.Tensor 
               out: torch.Tensor | None = None) -> torch.Tensor:
     """Rows back to tokens: y[t] = sum_s weights[t, s] * rows[topk_row[t, s]], fp32 in slot order, rounded once. weights
     bf16 / fp32 [N, k] or None (1). `combine` is the bf16 form without weights that the fused layer ends with.
-    Differentiable in rows and weights (without `out`)."""
+    Differentiable in rows and weights (without `out`); the gradient takes a plan that names no row twice, as route_pack's
+    (the sum itself takes any)."""
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
         if out is None:
             return _Unpermute.apply(rows, topk_row, weights)
