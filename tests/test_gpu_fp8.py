@@ -679,6 +679,59 @@ def test_layer_on_another_stream_and_in_two_graphs():
     assert fp8.status() == 0
 
 
+def test_layer_gradients_in_a_captured_graph():
+    """The layer's forward and backward captured once and replayed on other inputs and routes give the eager calls' bits."""
+    shape = SHAPES["odd"]
+    layer = _layer(shape)
+    n = 50
+
+    def step(x, idx, w, dy):
+        y = layer.forward_routed(x, idx, w)
+        return (y.detach(), *torch.autograd.grad(y, (x, w), dy))
+
+    def inputs(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        idx = torch.rand(n, shape.num_experts, generator=g, device="cuda").topk(shape.top_k, 1).indices.int()
+        return (torch.randn(n, shape.hidden, generator=g, device="cuda").bfloat16(), idx,
+                torch.rand(n, shape.top_k, generator=g, device="cuda"),
+                torch.randn(n, shape.hidden, generator=g, device="cuda").bfloat16())
+
+    def leaves(i):
+        return i[0].requires_grad_(), i[1], i[2].requires_grad_(), i[3]
+
+    fixed = leaves(inputs(0))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(*fixed)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*fixed)
+    for seed in (1, 2, 3):
+        new = inputs(seed)
+        with torch.no_grad():
+            for a, b in zip(fixed, new):
+                a.copy_(b)
+        graph.replay()
+        for a, b in zip(got, step(*leaves(new))):
+            assert torch.equal(a, b)
+    assert fp8.status() == 0
+
+
+def test_layer_takes_ids_outside_the_experts_as_none():
+    shape = SHAPES["flat"]
+    layer = _layer(shape)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(40, shape.hidden, generator=g, device="cuda").bfloat16()
+    idx = torch.rand(40, shape.num_experts, generator=g, device="cuda").topk(2, 1).indices.int()
+    w = torch.rand(40, 2, generator=g, device="cuda")
+    none, outside = idx.clone(), idx.clone()
+    none[::3, 1] = -1
+    outside[::3, 1] = torch.tensor([8, 9, 1000, -2, -2 ** 31, 2 ** 31 - 1, 8], device="cuda", dtype=torch.int32).repeat(2)
+    assert torch.equal(layer.forward_routed(x, outside, w), layer.forward_routed(x, none, w))
+
+
 def test_layer_refuses():
     layer = _layer(SHAPES["flat"])
     x = torch.randn(4, 512, device="cuda").bfloat16()
